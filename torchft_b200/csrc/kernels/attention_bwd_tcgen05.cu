@@ -40,12 +40,19 @@
 // zeros.  The statistics and the dQ accumulator are laid out for whole tiles; a query beyond the end has the log-sum-exp
 // +infinity there, so its probabilities are zero, and dQ, dK and dV beyond the end are not stored.
 //
+// With MASK a key is seen by a range of queries of its own (attention_masks.cuh), so a block walks over the query tiles of that range only, and
+// a softmax thread, whose key it is, holds the range's ends.  With SCORE the scores were capped or lowered by their distance, which is done
+// again here, and dS gets the factor 1 - tanh^2 by way of P, once dV's operand has been made of it.
+//
 // Every mbarrier wait is bounded; on expiry the CTA records FTB200_ST_TIMEOUT in the caller's
 // status word, frees its TMEM and returns.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <math.h>
 
+#include <initializer_list>
+
+#include "attention_masks.cuh"
 #include "ftb200_common.cuh"
 #include "tcgen05_helpers.cuh"
 
@@ -124,6 +131,7 @@ struct BwdParams {
   float4* dkv_part;    // split > 1: their dV and dK, fp32, per (batch, kv head, key block, share) [2][D / 4][128 keys][4]
   const float4* rope;  // null, or (cos, sin) pairs [seq][D / 2]: dQ and dK are rotated back
   int* status;
+  ftb200::MaskParams mask;  // of the kernels with MASK
 };
 
 // Eight elements (four pairs) rotated back by their angles (cos, sin, cos, sin).
@@ -149,7 +157,7 @@ __device__ __forceinline__ void bulk_add_f32(float* dst, uint32_t src, uint32_t 
                : "memory");
 }
 
-template <int D>
+template <int D, bool MASK, bool SCORE>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
@@ -184,14 +192,14 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   const int rep = p.n_heads / p.n_kv_heads / p.split;  // of this CTA
   const int h0 = (hk * p.split + share) * rep;
   const int n_qtiles = (p.seq + BQ - 1) / BQ;
-  const int first_q = p.causal ? jb : 0;
-  const int T = rep * (n_qtiles - first_q);
+  int first_q = p.causal ? jb : 0, end_q = n_qtiles;
+  int T = rep * (n_qtiles - first_q);
   // tiles in order: the queries of a head that see the block, then the next head of the group
   struct TileWalk {
     int h, qt;
   };
   auto next_tile = [&](TileWalk& w) {
-    if (++w.qt == n_qtiles) {
+    if (++w.qt == end_q) {
       w.qt = first_q;
       ++w.h;
     }
@@ -228,12 +236,18 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   ftb200::wait_for_previous();
+  if constexpr (MASK) {
+    const ftb200::KeyRange r = p.mask.queries_of(b, jb, p.seq);
+    first_q = r.lo / BQ;
+    end_q = r.hi > r.lo ? (r.hi + BQ - 1) / BQ : first_q;
+    T = rep * (end_q - first_q);
+  }
 
   if (warp < 4) {
     regs_dec<ISSUE_REGS>();
     if (warp == 0) {
       // ---------------- TMA producer ----------------
-      if (elect_one()) {
+      if (elect_one() && (!MASK || T > 0)) {
         mbar_expect_tx(bar(BAR_KV), 2 * TILE);
 #pragma unroll
         for (int sl = 0; sl < SLABS; ++sl) {
@@ -330,11 +344,25 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       };
       // S^T of the next tile is issued ahead of the products that wait for this tile's dS^T, so that its softmax runs
       // under them; the columns of S^T are free for it as P^T's reader, dV, was issued before.
-      bool ok = wait(BAR_KV, 0) && wait(BAR_Q_FULL, 0);
-      if (ok) score(Ly::COL_S, k_km, q_km0, BAR_S_FULL);
+      const bool padded = MASK && p.mask.has_padding(b);
+      TileWalk next{h0, first_q};  // the tile whose Q or dO is waited for
+      auto clear = [&](uint32_t off, int tile) {
+        if (padded) p.mask.clear_padding(smem + off, SLABS, b, tile, p.seq, lane);
+      };
+      bool ok = (!MASK || T > 0) && wait(BAR_KV, 0) && wait(BAR_Q_FULL, 0);
+      if (ok) {
+        clear(Ly::OFF_K, jb);
+        clear(Ly::OFF_V, jb);
+        clear(Ly::OFF_Q, first_q);
+        score(Ly::COL_S, k_km, q_km0, BAR_S_FULL);
+      }
       ok = ok && wait(BAR_DO_FULL, 0);
-      if (ok) score(Ly::COL_DP, v_km, do_km0, BAR_DP_FULL);
+      if (ok) {
+        clear(Ly::OFF_DO, first_q);
+        score(Ly::COL_DP, v_km, do_km0, BAR_DP_FULL);
+      }
       for (int t = 0; t < T && ok; ++t) {
+        if constexpr (MASK) next_tile(next);
         const int st = t % STAGES, nst = (t + 1) % STAGES;
         const uint32_t odd = static_cast<uint32_t>(t) & 1u, nph = static_cast<uint32_t>((t + 1) / STAGES) & 1u;
         const int dst = t % Ly::DO_STAGES, ndst = (t + 1) % Ly::DO_STAGES;
@@ -342,6 +370,7 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         from_tmem(Ly::COL_DV, Ly::COL_S, do_mn0 + dst * TILE16, t == 0, BAR_DO_EMPTY + dst);
         if (t + 1 < T) {
           if (!(ok = wait(BAR_Q_FULL + nst, nph))) break;
+          clear(Ly::OFF_Q + nst * TILE, next.qt);
           score(Ly::COL_S, k_km, q_km0 + nst * TILE16, BAR_S_FULL);
         }
         if (!(ok = wait(BAR_DS_READY, odd))) break;
@@ -356,6 +385,7 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         __syncwarp();
         if (t + 1 < T) {
           if (!(ok = wait(BAR_DO_FULL + ndst, static_cast<uint32_t>((t + 1) / Ly::DO_STAGES) & 1u))) break;
+          clear(Ly::OFF_DO + ndst * TILE, next.qt);
           if (Ly::DQ_OVER_DP && !(ok = wait(BAR_DQ_EMPTY, odd))) break;  // dQ^T of tile t drained
           score(Ly::COL_DP, v_km, do_km0 + ndst * TILE16, BAR_DP_FULL);
         }
@@ -422,6 +452,8 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     const uint32_t dp_addr = tmem_base + Ly::COL_DP + g * CPT + lane_addr;
     const bool beyond = jb * BKV + row >= p.seq;  // this key
     uint8_t* drow = smem + Ly::OFF_DS + g * SLAB + row * 128;
+    ftb200::RowMask mine = {0, 0, 0, 0};  // of the key: its queries
+    if constexpr (MASK) mine = p.mask.column(b, jb * BKV + row, p.seq);
     for (int t = 0; t < T && ok; ++t, next_tile(w)) {
       const uint32_t odd = static_cast<uint32_t>(t) & 1u;
       const int st = t % STAGES;
@@ -436,7 +468,45 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       const ulonglong2* lse2 = reinterpret_cast<const ulonglong2*>(smem + Ly::OFF_STATS + st * STATS_BYTES) + g * (CPT / 4);
       const ulonglong2* delta2 = lse2 + BQ / 4;
       float pe[CPT];
-      {
+      if constexpr (SCORE) {
+        uint32_t sv[CPT];
+        tmem_ld32(s_addr, sv);
+        tmem_ld32(s_addr + 32, sv + 32);
+        tmem_wait_ld();
+        p.mask.cap_scores<CPT>(sv);
+        const float slope2 = p.mask.slope2(w.h);
+        const float far = static_cast<float>(w.qt * BQ + g * CPT - (jb * BKV + row));
+        const bool all = mine.all(w.qt * BQ, BQ);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int q0 = w.qt * BQ + g * CPT + half * 32;
+          const uint32_t bits = all ? 0xffffffffu : ftb200::range_bits(mine.lo - q0, mine.hi - q0);
+          uint32_t pt[16];
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            const int qi = half * 32 + 2 * c;
+            const ulonglong2 l4 = lse2[qi / 4];
+            float y0 = __uint_as_float(sv[qi]), y1 = __uint_as_float(sv[qi + 1]), x0, x1;
+            f2_unpack(f2_add(f2_pack(y0, y1), c % 2 == 0 ? l4.x : l4.y), x0, x1);
+            if (p.mask.slopes != nullptr) {
+              x0 = fmaf(-slope2, fabsf(far + qi), x0);
+              x1 = fmaf(-slope2, fabsf(far + (qi + 1)), x1);
+            }
+            x0 = bits >> (2 * c) & 1u ? exp2f(x0) : 0.f;
+            x1 = bits >> (2 * c + 1) & 1u ? exp2f(x1) : 0.f;
+            __nv_bfloat162 a = __floats2bfloat162_rn(x0, x1);
+            pt[c] = *reinterpret_cast<uint32_t*>(&a);
+            if (p.mask.capped) {
+              x0 *= fmaf(y0 * p.mask.neg_inv_cap2_sq, y0, 1.f);
+              x1 *= fmaf(y1 * p.mask.neg_inv_cap2_sq, y1, 1.f);
+            }
+            pe[qi] = x0;
+            pe[qi + 1] = x1;
+          }
+          tmem_st16(s_addr + half * 16, pt);  // over scores that this thread has read
+        }
+        tmem_wait_st();
+      } else {
         uint32_t sv[CPT];
         tmem_ld32(s_addr, sv);
         tmem_ld32(s_addr + 32, sv + 32);
@@ -455,7 +525,18 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           }
         }
       }
-      if (p.causal != 0 && w.qt == jb) {  // the diagonal tile: queries before the key
+      if constexpr (MASK) {
+        if (!SCORE && !mine.all(w.qt * BQ, BQ)) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int q0 = w.qt * BQ + g * CPT + half * 32;
+            const uint32_t bits = ftb200::range_bits(mine.lo - q0, mine.hi - q0);
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (!(bits >> c & 1u)) pe[half * 32 + c] = 0.f;
+          }
+        }
+      } else if (p.causal != 0 && w.qt == jb) {  // the diagonal tile: queries before the key
 #pragma unroll
         for (int c = 0; c < CPT; ++c)
           if (row > g * CPT + c) pe[c] = 0.f;
@@ -463,7 +544,7 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 #pragma unroll
         for (int c = 0; c < CPT; ++c) pe[c] = 0.f;
       }
-      {
+      if constexpr (!SCORE) {
         uint32_t pt[CPT / 2];
 #pragma unroll
         for (int c = 0; c < CPT / 2; ++c) {
@@ -518,7 +599,8 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       tc_fence_before();
       mbar_arrive_warp(bar(BAR_DS_READY));
     }
-    if (ok && mbar_wait_warp(bar(BAR_DKV_DONE), 0, abort_flag)) {
+    const bool unseen = MASK && T == 0;  // by every query: zeros
+    if (ok && (unseen || mbar_wait_warp(bar(BAR_DKV_DONE), 0, abort_flag))) {
       tc_fence_after();
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
@@ -531,6 +613,10 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 #pragma unroll
         for (int c = 0; c < CW / 32; ++c) tmem_ld32(tmem_base + col + c * 32 + lane_addr, v + c * 32);
         tmem_wait_ld();
+        if (unseen) {
+#pragma unroll
+          for (int c = 0; c < CW; ++c) v[c] = 0u;
+        }
         if (p.split > 1) {
           float4* part = p.dkv_part + ((static_cast<long long>(bh) * n_qtiles + jb) * p.split + share) * (2 * D / 4 * BKV) +
                          (which * D / 4 + g * CW / 4) * BKV + row;
@@ -603,8 +689,10 @@ __global__ void __launch_bounds__(256) attention_bwd_prep_kernel(const __nv_bflo
   for (int k = LANES / 2; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
   if (live && c % LANES == 0) {
     const long long bh = static_cast<long long>(b) * n_heads + c / LANES;
-    neg_delta[bh * seq_t + pos] = inside ? -s * scale : 0.f;
-    neg_lse2[bh * seq_t + pos] = inside ? lse[bh * seq + pos] * -1.4426950408889634f : -INFINITY;
+    // a query that saw nothing (a mask's doing) has a log-sum-exp of -infinity; its output and dO may be anything
+    const float l = inside ? lse[bh * seq + pos] : -INFINITY;
+    neg_delta[bh * seq_t + pos] = l != -INFINITY ? -s * scale : 0.f;
+    neg_lse2[bh * seq_t + pos] = l != -INFINITY ? l * -1.4426950408889634f : -INFINITY;
   }
 }
 
@@ -765,12 +853,13 @@ FTB200_API long long ftb200_attention_bwd_scratch_bytes(int batch, int seq, int 
 
 namespace {
 
-template <int D>
+template <int D, bool MASK, bool SCORE>
 int attention_bwd_impl(const void* q, const void* k, const void* v, const void* o, const void* d_o, const float* lse,
                        void* dq, void* dk, void* dv, void* scratch, int batch, int seq, int n_heads, int n_kv_heads,
                        long long ld_q, long long ld_k, long long ld_v, long long ld_o, long long ld_do, long long ld_dq,
                        long long ld_dk, long long ld_dv, float scale, int causal, const float* cos_sin, int* status,
-                       cudaStream_t stream) {
+                       const ftb200::MaskParams& mask, cudaStream_t stream) {
+  auto* kernel = attention_bwd_kernel<D, MASK, SCORE>;
   constexpr uint32_t SMEM_BYTES = Lay<D>::SMEM_BYTES;
   const long long tiles = (static_cast<long long>(seq) + BQ - 1) / BQ;
   const long long rows = batch * tiles * BQ;
@@ -787,12 +876,11 @@ int attention_bwd_impl(const void* q, const void* k, const void* v, const void* 
   if (rc != 0) return rc;
   static bool attr_set = false;
   if (!attr_set) {
-    if (cudaFuncSetAttribute(attention_bwd_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) !=
-        cudaSuccess)
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess)
       return FTB200_E_CUDA;
     // the warpgroups share out what a CTA is launched with: with fewer registers a thread the increase would wait for good
     cudaFuncAttributes attr;
-    if (cudaFuncGetAttributes(&attr, attention_bwd_kernel<D>) != cudaSuccess) return FTB200_E_CUDA;
+    if (cudaFuncGetAttributes(&attr, kernel) != cudaSuccess) return FTB200_E_CUDA;
     if (attr.numRegs < LAUNCH_REGS) return FTB200_E_REGS;
     attr_set = true;
   }
@@ -801,7 +889,7 @@ int attention_bwd_impl(const void* q, const void* k, const void* v, const void* 
   ftb200::launch_after(attention_bwd_prep_kernel<D>, static_cast<unsigned>((pieces + 255) / 256), 256, 0, stream,
       reinterpret_cast<const __nv_bfloat16*>(o), reinterpret_cast<const __nv_bfloat16*>(d_o), lse, neg_lse2, neg_delta,
       reinterpret_cast<float4*>(dq_acc), seq, n_heads, pieces, ld_o, ld_do, scale);
-  BwdParams p;
+  BwdParams p = {};
   p.batch = batch; p.seq = seq; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads; p.causal = causal;
   p.scale = scale; p.scale_log2 = scale * 1.4426950408889634f;
   p.neg_lse2 = neg_lse2; p.neg_delta = neg_delta; p.dq_acc = dq_acc;
@@ -809,10 +897,11 @@ int attention_bwd_impl(const void* q, const void* k, const void* v, const void* 
   p.ld_dk = ld_dk; p.ld_dv = ld_dv; p.status = status;
   p.rope = reinterpret_cast<const float4*>(cos_sin);
   p.split = split;
+  p.mask = mask;
   p.dkv_part = reinterpret_cast<float4*>(neg_lse2 + rows * n_heads);
   const long long grid = static_cast<long long>(batch) * n_kv_heads * tiles * split;
   if (grid > 0x7fffffffLL) return FTB200_E_TOOBIG;
-  ftb200::launch_after(attention_bwd_kernel<D>, static_cast<unsigned>(grid), NUM_THREADS, SMEM_BYTES, stream, tq, tk, tv, tdo,
+  ftb200::launch_after(kernel, static_cast<unsigned>(grid), NUM_THREADS, SMEM_BYTES, stream, tq, tk, tv, tdo,
       p);
   const long long cast_warps = batch * tiles * n_heads * (D / 64) * (32 / CAST_GROUPS);
   const long long dkv_blocks = split > 1 ? static_cast<long long>(batch) * n_kv_heads * tiles * (2 * D / 32) : 0;
@@ -821,6 +910,18 @@ int attention_bwd_impl(const void* q, const void* k, const void* v, const void* 
       reinterpret_cast<const float4*>(dq_acc), reinterpret_cast<__nv_bfloat16*>(dq), cast_warps, ld_dq,
       static_cast<int>(dkv_blocks), p);
   return cudaGetLastError() == cudaSuccess ? 0 : FTB200_E_CUDA;
+}
+
+int check_bwd(const void* q, const void* k, const void* v, const void* o, const void* d_o, const void* dq, const void* dk, const void* dv,
+              const void* scratch, const void* cos_sin, int batch, int seq, int n_heads, int n_kv_heads, int head_dim,
+              std::initializer_list<long long> lds) {
+  if ((head_dim != 64 && head_dim != 128) || batch <= 0 || seq <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0)
+    return FTB200_E_BADARG;
+  for (const void* x : {q, k, v, o, d_o, dq, dk, dv, scratch, cos_sin})
+    if (!aligned16(x)) return FTB200_E_ALIGN;
+  for (long long x : lds)
+    if (x & 7) return FTB200_E_ALIGN;
+  return 0;
 }
 
 }  // namespace
@@ -836,18 +937,29 @@ FTB200_API int ftb200_attention_bwd(const void* q, const void* k, const void* v,
                                     long long ld_v, long long ld_o, long long ld_do, long long ld_dq, long long ld_dk,
                                     long long ld_dv, float scale, int causal, const float* cos_sin, int* status,
                                     cudaStream_t stream) {
-  if ((head_dim != 64 && head_dim != 128) || batch <= 0 || seq <= 0 || n_heads <= 0 ||
-      n_kv_heads <= 0 || n_heads % n_kv_heads != 0)
-    return FTB200_E_BADARG;
-  const void* ptrs[] = {q, k, v, o, d_o, dq, dk, dv, scratch, cos_sin};
-  for (const void* x : ptrs)
-    if (!aligned16(x)) return FTB200_E_ALIGN;
-  const long long lds[] = {ld_q, ld_k, ld_v, ld_o, ld_do, ld_dq, ld_dk, ld_dv};
-  for (long long x : lds)
-    if (x & 7) return FTB200_E_ALIGN;
-  if (head_dim == 64)
-    return attention_bwd_impl<64>(q, k, v, o, d_o, lse, dq, dk, dv, scratch, batch, seq, n_heads, n_kv_heads, ld_q, ld_k,
-                                  ld_v, ld_o, ld_do, ld_dq, ld_dk, ld_dv, scale, causal, cos_sin, status, stream);
-  return attention_bwd_impl<128>(q, k, v, o, d_o, lse, dq, dk, dv, scratch, batch, seq, n_heads, n_kv_heads, ld_q, ld_k,
-                                 ld_v, ld_o, ld_do, ld_dq, ld_dk, ld_dv, scale, causal, cos_sin, status, stream);
+  const int rc = check_bwd(q, k, v, o, d_o, dq, dk, dv, scratch, cos_sin, batch, seq, n_heads, n_kv_heads, head_dim,
+                           {ld_q, ld_k, ld_v, ld_o, ld_do, ld_dq, ld_dk, ld_dv});
+  if (rc != 0) return rc;
+  return (head_dim == 64 ? attention_bwd_impl<64, false, false> : attention_bwd_impl<128, false, false>)(
+      q, k, v, o, d_o, lse, dq, dk, dv, scratch, batch, seq, n_heads, n_kv_heads, ld_q, ld_k, ld_v, ld_o, ld_do, ld_dq, ld_dk, ld_dv, scale, causal,
+      cos_sin, status, ftb200::MaskParams(), stream);
+}
+
+// The same under a mask, with the arguments of ftb200_attention_masked_fwd.
+FTB200_API int ftb200_attention_masked_bwd(const void* q, const void* k, const void* v, const void* o, const void* d_o, const float* lse, void* dq,
+                                           void* dk, void* dv, void* scratch, const void* rows, const void* tiles, const int* padded,
+                                           const float* slopes, int batch, int seq, int n_heads, int n_kv_heads, int head_dim, long long ld_q,
+                                           long long ld_k, long long ld_v, long long ld_o, long long ld_do, long long ld_dq, long long ld_dk,
+                                           long long ld_dv, float scale, float softcap, int causal, const float* cos_sin, int* status,
+                                           cudaStream_t stream) {
+  int rc = check_bwd(q, k, v, o, d_o, dq, dk, dv, scratch, cos_sin, batch, seq, n_heads, n_kv_heads, head_dim,
+                     {ld_q, ld_k, ld_v, ld_o, ld_do, ld_dq, ld_dk, ld_dv});
+  ftb200::MaskParams mask = {};
+  if (rc == 0) rc = ftb200::set_mask(&mask, rows, tiles, padded, slopes, scale, softcap, causal, seq);
+  if (rc != 0) return rc;
+  auto* impl = softcap > 0.f || slopes != nullptr
+                   ? (head_dim == 64 ? attention_bwd_impl<64, true, true> : attention_bwd_impl<128, true, true>)
+                   : (head_dim == 64 ? attention_bwd_impl<64, true, false> : attention_bwd_impl<128, true, false>);
+  return impl(q, k, v, o, d_o, lse, dq, dk, dv, scratch, batch, seq, n_heads, n_kv_heads, ld_q, ld_k, ld_v, ld_o, ld_do, ld_dq, ld_dk, ld_dv, scale,
+              causal, cos_sin, status, mask, stream);
 }

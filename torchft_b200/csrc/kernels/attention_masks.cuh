@@ -1,0 +1,207 @@
+// Masks and score changes of the attention kernels.
+//
+// What a query sees is one range of keys [lo, hi), and who sees a key one range of queries [from, to) (packed_rows.cu: documents, prefixes,
+// windows, padding).  A tile of 128 queries then has one range of key blocks to look at, a block that each of its queries sees needs no
+// mask, and in any other the seen keys of a row are a run of bits.
+//
+// A score s (the product of query and key) becomes
+//
+//   y = log2(e) (softcap tanh(scale s / softcap) - slope |query - key|)
+//
+// tanh(x) is x P(x^2) up to |x| = 0.8, where P of degree 5 has a relative error of 5.8e-8 (least largest error, by Lawson's iteration of weighted
+// least squares): seven operations of the FMA pipe, with scale and cap inside the coefficients, while the exponential unit, which the softmax
+// wants for itself, stays free.  A thread's scores that go beyond take 1 - 2 / (exp(2x) + 1), with an error of about 1e-7 of the cap, which
+// is what counts in a score.
+#pragma once
+
+#include <limits.h>
+#include <math.h>
+
+#include "ftb200_common.cuh"
+#include "tcgen05_helpers.cuh"
+
+namespace ftb200 {
+
+// Bits [a, b) of a word; a and b may lie outside of it.
+__device__ __forceinline__ uint32_t range_bits(int a, int b) {
+  const uint32_t below_b = b <= 0 ? 0u : b >= 32 ? 0xffffffffu : (1u << b) - 1u;
+  const uint32_t below_a = a <= 0 ? 0u : a >= 32 ? 0xffffffffu : (1u << a) - 1u;
+  return below_b & ~below_a;
+}
+
+struct KeyRange {
+  int lo, hi;
+};
+
+// A query's keys [lo, hi), and the keys [all_lo, all_hi) that every query of its tile sees.
+struct RowMask {
+  int lo, hi, all_lo, all_hi;
+  __device__ __forceinline__ bool all(int first, int n) const { return all_lo <= first && first + n <= all_hi; }
+};
+
+struct MaskParams {
+  const int4* rows;  // null, or [batch][seq]: lo, hi, from, to
+  const int4* tiles;  // [batch][tiles of 128][2]: (lo, hi, all_lo, all_hi), (from, to, all_from, all_to)
+  const int* padded;  // [batch]: whether a row has padding
+  int causal;         // without rows
+  int capped;
+  const float* slopes;  // null, or [heads]
+  float scale_log2;     // log2(e) scale
+  float poly[6];        // of s^2: y = s P(s^2)
+  float poly_up_to;     // |s| that it holds for
+  float cap2;           // log2(e) softcap
+  float in2;            // 2 log2(e) scale / softcap
+  float neg_inv_cap2_sq;  // -1 / cap2^2: 1 - tanh^2 = 1 + y^2 times this
+
+  __device__ __forceinline__ int4 tile(int b, int t, int seq, int which) const {
+    return tiles[(static_cast<long long>(b) * ((seq + 127) / 128) + t) * 2 + which];
+  }
+
+  // Keys that the `n` tiles of 128 queries from q0 on look at.
+  __device__ __forceinline__ KeyRange keys_of(int b, int q0, int n, int seq) const {
+    if (rows == nullptr) return {0, causal ? min(seq, q0 + n * 128) : seq};
+    KeyRange r = {INT_MAX, 0};
+    for (int t = 0; t < n && q0 + t * 128 < seq; ++t) {
+      const int4 x = tile(b, q0 / 128 + t, seq, 0);
+      r.lo = min(r.lo, x.x);
+      r.hi = max(r.hi, x.y);
+    }
+    return r;
+  }
+
+  __device__ __forceinline__ RowMask row(int b, int query, int seq) const {
+    RowMask m = {0, 0, INT_MAX, 0};
+    if (query >= seq) return m;
+    if (rows == nullptr) {
+      m.hi = causal ? query + 1 : seq;
+      m.all_lo = 0;
+      m.all_hi = causal ? query / 128 * 128 + 1 : seq;
+      return m;
+    }
+    const int4 r = rows[static_cast<long long>(b) * seq + query];
+    const int4 x = tile(b, query / 128, seq, 0);
+    return {r.x, r.y, x.z, x.w};
+  }
+
+  // The other way round: the queries that the block of 128 keys looks at, and those that see a key.
+  __device__ __forceinline__ KeyRange queries_of(int b, int t, int seq) const {
+    if (rows == nullptr) return {causal ? t * 128 : 0, seq};
+    const int4 x = tile(b, t, seq, 1);
+    return {x.x, x.y};
+  }
+
+  __device__ __forceinline__ RowMask column(int b, int key, int seq) const {
+    RowMask m = {0, 0, INT_MAX, 0};
+    if (key >= seq) return m;
+    if (rows == nullptr) {
+      m.lo = causal ? key : 0;
+      m.hi = seq;
+      if ((key | 127) < seq) {
+        m.all_lo = causal ? key | 127 : 0;
+        m.all_hi = seq;
+      }
+      return m;
+    }
+    const int4 r = rows[static_cast<long long>(b) * seq + key];
+    const int4 x = tile(b, key / 128, seq, 1);
+    return {r.z, r.w, x.z, x.w};
+  }
+
+  __device__ __forceinline__ bool has_padding(int b) const { return rows != nullptr && padded[b] != 0; }
+
+  // Rows of a tile in shared memory (slabs of 128 rows x 128 bytes) that belong to padding become zeros, by one warp: what stands in padding may
+  // be anything, and zero times infinity would reach the tile's other rows.  The products that follow see it.
+  __device__ __forceinline__ void clear_padding(uint8_t* tile_mem, int slabs, int b, int t, int seq, int lane) const {
+    if (tile(b, t, seq, 0).z != INT_MAX) return;
+    for (int r = lane; r < 128 && t * 128 + r < seq; r += 32) {
+      const int4 x = rows[static_cast<long long>(b) * seq + t * 128 + r];
+      if (x.y > x.x) continue;
+      for (int s = 0; s < slabs; ++s)
+        for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(tile_mem + s * (128 * 128) + r * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    tc::fence_async_smem();
+    __syncwarp();
+  }
+
+  __device__ __forceinline__ float slope2(int head) const { return slopes == nullptr ? 0.f : slopes[head] * 1.4426950408889634f; }
+
+  // A thread's N products become log2(e) softcap tanh(scale s / softcap), or log2(e) scale s without a cap.
+  template <int N>
+  __device__ __forceinline__ void cap_scores(uint32_t* sv) const {
+    using namespace tc;
+    if (capped) {
+      float big[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < N; c += 2)
+        big[(c >> 1) & 3] = fmaxf(fmaxf(big[(c >> 1) & 3], fabsf(__uint_as_float(sv[c]))), fabsf(__uint_as_float(sv[c + 1])));
+      if (__all_sync(0xffffffffu, fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) <= poly_up_to)) {
+        unsigned long long k[6];
+#pragma unroll
+        for (int i = 0; i < 6; ++i) k[i] = f2_pack(poly[i], poly[i]);
+#pragma unroll
+        for (int c = 0; c < N; c += 2) {
+          const unsigned long long s = f2_pack(__uint_as_float(sv[c]), __uint_as_float(sv[c + 1]));
+          const unsigned long long u = f2_mul(s, s);
+          unsigned long long y = f2_fma(u, k[5], k[4]);
+#pragma unroll
+          for (int i = 3; i >= 0; --i) y = f2_fma(u, y, k[i]);
+          float y0, y1;
+          f2_unpack(f2_mul(s, y), y0, y1);
+          sv[c] = __float_as_uint(y0);
+          sv[c + 1] = __float_as_uint(y1);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+          const float e = exp2f(__uint_as_float(sv[c]) * in2);
+          sv[c] = __float_as_uint(fmaf(-2.f * cap2, __frcp_rn(e + 1.f), cap2));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < N; ++c) sv[c] = __float_as_uint(__uint_as_float(sv[c]) * scale_log2);
+    }
+  }
+
+  // The slope's part, for score c at the distance |far + c step| (step 1 or -1).
+  template <int N>
+  __device__ __forceinline__ void slope_scores(uint32_t* sv, float far, float step, float slope2) const {
+    if (slopes == nullptr) return;
+#pragma unroll
+    for (int c = 0; c < N; ++c) sv[c] = __float_as_uint(fmaf(-slope2, fabsf(far + c * step), __uint_as_float(sv[c])));
+  }
+};
+
+inline int set_mask(MaskParams* m, const void* rows, const void* tiles, const int* padded, const float* slopes, float scale, float softcap, int causal,
+                    int seq) {
+  if ((rows != nullptr) != (tiles != nullptr) || (rows != nullptr) != (padded != nullptr) || !(softcap >= 0.f) || !(softcap < INFINITY))
+    return FTB200_E_BADARG;
+  if ((reinterpret_cast<uintptr_t>(rows) & 15) || (reinterpret_cast<uintptr_t>(tiles) & 15)) return FTB200_E_ALIGN;
+  if (seq > (1 << 30)) return FTB200_E_TOOBIG;
+  constexpr double LOG2E = 1.4426950408889634;
+  m->rows = static_cast<const int4*>(rows);
+  m->tiles = static_cast<const int4*>(tiles);
+  m->padded = padded;
+  m->causal = causal;
+  m->slopes = slopes;
+  m->capped = softcap > 0.f;
+  m->scale_log2 = static_cast<float>(scale * LOG2E);
+  if (softcap > 0.f) {
+    constexpr double P[6] = {0.9999999420836679, -0.333326749210523, 0.1332104829082429, -0.05311431573861419, 0.01909330062970014,
+                             -0.004355299563624438};
+    const double k = static_cast<double>(scale) / softcap, cap2 = softcap * LOG2E;
+    double power = cap2 * k;
+    bool fits = true;
+    for (int i = 0; i < 6; ++i, power *= k * k) {
+      m->poly[i] = static_cast<float>(P[i] * power);
+      fits = fits && isfinite(m->poly[i]);
+    }
+    m->poly_up_to = fits ? static_cast<float>(0.8 / k) : -1.f;
+    m->cap2 = static_cast<float>(cap2);
+    m->in2 = static_cast<float>(2.0 * LOG2E * k);
+    m->neg_inv_cap2_sq = static_cast<float>(-1.0 / (cap2 * cap2));
+  }
+  return 0;
+}
+
+}  // namespace ftb200

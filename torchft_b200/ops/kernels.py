@@ -15,7 +15,7 @@ import ctypes
 import functools
 import math
 import os
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple
 
 import torch
 import torch.nn.functional as F
@@ -57,6 +57,9 @@ _ARGS = {
     "cross_entropy": "pppiilfip", "adamw": "ppppiplfffffipp", "sumsq": "pilpp", "clip_coef": "pfppp",
     "attention_fwd": "pppppiiiiillllfipp", "attention_fwd2": "pppppiiiiillllfiipp",
     "attention_bwd": "ppppppppppiiiiillllllllfippp", "gemm_bf16": "pppiiiiilllipip",
+    "attention_spans": "ppppppiiiip", "attention_masked_fwd": "pppppppppiiiiillllffipp",
+    "attention_masked_bwd": "ppppppppppppppiiiiillllllllffippp", "rope_axes": "ppppliiiliiip",
+    "layernorm_fwd": "pppppppplifip", "layernorm_bwd": "ppppppppppliiip",
 }
 _ARGS["gemm_bf16_2cta"] = _ARGS["gemm_bf16"]
 _KIND = {"p": c_void_p, "i": c_int, "l": c_ll, "f": c_float}
@@ -381,6 +384,161 @@ def rmsnorm_bwd(
     return dx, dw
 
 
+# --------------------------------------------------------------------------- layer norm
+
+
+def _check_here(named) -> None:
+    """The tensors are on the current device, whose stream the kernel is launched on."""
+    device = next(t for _, t in named if t is not None).device
+    for name, t in named:
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if device.type == "cuda" and device.index != torch._C._cuda_getDevice():
+        raise ValueError(f"the tensors are on {device}, which is not the current device")
+
+
+def _check_rows(named, dtype: torch.dtype) -> None:
+    for name, t, shape in named:
+        if t is not None and (t.dtype != dtype or t.shape != shape or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous {dtype} of shape {tuple(shape)}, got {t.dtype} of {tuple(t.shape)}")
+
+
+def _check_norm(x: torch.Tensor) -> None:
+    if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float32) or x.shape[1] % 8 or x.shape[1] == 0:
+        raise ValueError("x must be [rows, width] in bf16 or fp32 with a width that is a multiple of 8")
+
+
+def ref_layernorm_fwd(x, w, b=None, eps=1e-5, res=None):
+    h = x.float()
+    if res is not None:
+        h = (h + res.float()).to(x.dtype).float()
+    mean = h.mean(-1)
+    c = h - mean.unsqueeze(-1)
+    rstd = torch.rsqrt(c.pow(2).mean(-1) + eps)
+    y = c * rstd.unsqueeze(-1) * w.float()
+    return (y if b is None else y + b.float()).to(x.dtype), mean, rstd, h.to(x.dtype)
+
+
+def layernorm_fwd(
+    x: torch.Tensor,
+    w: torch.Tensor,
+    b: Optional[torch.Tensor] = None,
+    eps: float = 1e-5,
+    res: Optional[torch.Tensor] = None,
+    h_out: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+    mean: Optional[torch.Tensor] = None,
+    rstd: Optional[torch.Tensor] = None,
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Returns ``(normed, mean, rstd, h)`` where ``h = x + res`` (or ``x``), rounded to the type of ``x``, and ``normed = (h - mean) *
+    rstd * w (+ b)``.  Rows of up to 16384 elements, all tensors in bf16 or all in fp32 (``mean`` and ``rstd`` in fp32).  ``out`` and
+    ``h_out`` may be ``x`` or ``res``."""
+    _check_norm(x)
+    T, D = x.shape
+    if mean is None:
+        mean = torch.empty(T, dtype=torch.float32, device=x.device)
+    if rstd is None:
+        rstd = torch.empty(T, dtype=torch.float32, device=x.device)
+    if res is not None and h_out is None:
+        h_out = torch.empty_like(x)
+    if out is None:
+        out = torch.empty_like(x)
+    _check_rows((("x", x, x.shape), ("w", w, (D,)), ("b", b, (D,)), ("res", res, x.shape), ("h_out", h_out, x.shape), ("out", out, x.shape)),
+                x.dtype)
+    _check_rows((("mean", mean, (T,)), ("rstd", rstd, (T,))), torch.float32)
+    _check_here((("x", x), ("w", w), ("b", b), ("res", res), ("h_out", h_out), ("out", out), ("mean", mean), ("rstd", rstd)))
+    if out is h_out and res is not None:
+        raise ValueError("out and h_out are two results")
+    if T > 0:
+        if not x.is_cuda:
+            o, m, r, h = ref_layernorm_fwd(x, w, b, eps, res)
+            out.copy_(o)
+            mean.copy_(m)
+            rstd.copy_(r)
+            if res is not None:
+                h_out.copy_(h)
+        else:
+            N.check(_fn("layernorm_fwd")(_at(x), _at(res), _at(h_out) if res is not None else None, _at(w), _at(b), _at(out), _at(mean),
+                                         _at(rstd), T, D, eps, int(x.dtype == torch.float32), _stream()), "layernorm_fwd")
+    return out, mean, rstd, h_out if res is not None else x
+
+
+def ref_layernorm_bwd(dy, x, w, mean, rstd, dres=None):
+    xh = (x.float() - mean.unsqueeze(-1)) * rstd.unsqueeze(-1)
+    dyf = dy.float()
+    g = dyf * w.float()
+    dx = rstd.unsqueeze(-1) * (g - g.mean(-1, keepdim=True) - xh * (g * xh).mean(-1, keepdim=True))
+    if dres is not None:
+        dx = dx + dres.float()
+    return dx.to(x.dtype), (dyf * xh).sum(0), dyf.sum(0)
+
+
+@functools.lru_cache(maxsize=256)
+def layernorm_bwd_scratch_floats(dim: int) -> int:
+    """Size of the ``scratch`` that :func:`layernorm_bwd` takes."""
+    lib = N.lib()
+    lib.ftb200_layernorm_bwd_scratch_floats.restype = c_ll
+    return int(lib.ftb200_layernorm_bwd_scratch_floats(dim))
+
+
+def layernorm_bwd(
+    dy: torch.Tensor,
+    x: torch.Tensor,
+    w: torch.Tensor,
+    mean: torch.Tensor,
+    rstd: torch.Tensor,
+    dres: Optional[torch.Tensor] = None,
+    dx: Optional[torch.Tensor] = None,
+    dw: Optional[torch.Tensor] = None,
+    db: Optional[torch.Tensor] = None,
+    bias: bool = True,
+    accumulate: bool = False,
+    scratch: Optional[torch.Tensor] = None,
+) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+    """``(dx, dw, db)`` of :func:`layernorm_fwd`, whose ``h`` is ``x`` here; ``db`` is None without ``bias``.  ``dres`` is added to ``dx``,
+    which may be ``dy``, ``x`` or ``dres``; with ``accumulate`` the sums are added to what ``dw`` and ``db`` hold.  The partial sums lie in
+    ``scratch`` (fp32 on the device, :func:`layernorm_bwd_scratch_floats` of them or more) between the two kernels, by default in memory
+    of this call's own."""
+    _check_norm(x)
+    T, D = x.shape
+    if accumulate and (dw is None or (bias and db is None)):
+        raise ValueError("accumulate needs dw and db")
+    if dx is None:
+        dx = torch.empty_like(x)
+    if dw is None:
+        dw = torch.empty_like(w)
+    if not bias:
+        db = None
+    elif db is None:
+        db = torch.empty_like(w)
+    _check_rows((("x", x, x.shape), ("dy", dy, x.shape), ("w", w, (D,)), ("dres", dres, x.shape), ("dx", dx, x.shape), ("dw", dw, (D,)),
+                 ("db", db, (D,))), x.dtype)
+    _check_rows((("mean", mean, (T,)), ("rstd", rstd, (T,))), torch.float32)
+    _check_here((("x", x), ("dy", dy), ("w", w), ("mean", mean), ("rstd", rstd), ("dres", dres), ("dx", dx), ("dw", dw), ("db", db),
+                 ("scratch", scratch)))
+    if T == 0:
+        if not accumulate:
+            dw.zero_()
+            if db is not None:
+                db.zero_()
+        return dx, dw, db
+    if not x.is_cuda:
+        rdx, rdw, rdb = ref_layernorm_bwd(dy, x, w, mean, rstd, dres)
+        dx.copy_(rdx)
+        dw.copy_(((dw.float() if accumulate else 0) + rdw).to(dw.dtype))
+        if db is not None:
+            db.copy_(((db.float() if accumulate else 0) + rdb).to(db.dtype))
+        return dx, dw, db
+    need = layernorm_bwd_scratch_floats(D)
+    if scratch is None:
+        scratch = torch.empty(need, dtype=torch.float32, device=x.device)
+    elif scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < need or scratch.data_ptr() % 16:
+        raise ValueError(f"scratch must be {need} contiguous fp32 on {x.device}")
+    N.check(_fn("layernorm_bwd")(_at(dy), _at(x), _at(w), _at(mean), _at(rstd), _at(dres), _at(dx), _at(dw), _at(db), _at(scratch), T, D,
+                                 int(accumulate), int(x.dtype == torch.float32), _stream()), "layernorm_bwd", launches=2)
+    return dx, dw, db
+
+
 # --------------------------------------------------------------------------- RoPE
 
 
@@ -417,6 +575,66 @@ def rope_(buf: torch.Tensor, table: torch.Tensor, seq_len: int, n_heads: int, he
         _fn("rope")(_at(buf), _at(table), T, seq_len, n_heads, head_dim, buf.stride(0), int(backward), _stream()),
         "rope",
     )
+    return buf
+
+
+def rope_axes_freqs(sections: Sequence[int], theta: float, device, restart: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``(inv_freq, axis)`` of :func:`rope_axes_` for a head whose first ``sections[0]`` pairs turn with the positions of axis 0, the next
+    ``sections[1]`` with those of axis 1, and so on (time, height, width).  The frequencies fall from 1 to ``1 / theta`` over all pairs,
+    or with ``restart`` over each section's own."""
+    if not sections or any(n < 0 for n in sections) or sum(sections) == 0:
+        raise ValueError("sections must be numbers of pairs, one per axis")
+    total = sum(sections)
+    inv, axis = [], []
+    for a, n in enumerate(sections):
+        at = torch.arange(n, dtype=torch.float64) / max(n, 1) if restart else (len(axis) + torch.arange(n, dtype=torch.float64)) / total
+        inv.append(theta ** -at)
+        axis += [a] * n
+    return torch.cat(inv).to(device), torch.tensor(axis, dtype=torch.int32, device=device)
+
+
+def ref_rope_axes(buf, positions, inv_freq, axis, n_heads, head_dim, half=False, backward=False):
+    T, axes = buf.shape[0], positions.shape[0]
+    turned = (axis >= 0) & (axis < axes)
+    pos = positions.double()[axis.long().clamp(0, axes - 1)].t()  # [T, pairs]
+    ang = torch.where(turned, pos * inv_freq, 0.0)
+    c, s = ang.cos().float()[:, None], ang.sin().float()[:, None]
+    if backward:
+        s = -s
+    rot = buf[:, : n_heads * head_dim].float().reshape(T, n_heads, head_dim)
+    x, y = (rot[..., : head_dim // 2], rot[..., head_dim // 2 :]) if half else (rot[..., 0::2], rot[..., 1::2])
+    a, b = x * c - y * s, x * s + y * c
+    o = torch.cat([a, b], -1) if half else torch.stack([a, b], -1)
+    res = buf.clone()
+    res[:, : n_heads * head_dim] = o.reshape(T, n_heads * head_dim).to(buf.dtype)
+    return res
+
+
+def rope_axes_(buf: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, axis: torch.Tensor, n_heads: int, head_dim: int,
+               half: bool = False, backward: bool = False) -> torch.Tensor:
+    """Rotate the first ``n_heads`` heads of every row of ``buf`` ``[T, >= n_heads*head_dim]`` (bf16 or fp32) in place by positions that
+    the rows bring along: pair ``j`` of a head turns by ``positions[axis[j], t] * inv_freq[j]`` (``positions`` int32 ``[axes, T]``,
+    ``inv_freq`` fp64 and ``axis`` int32, both ``[head_dim/2]``, see :func:`rope_axes_freqs`); an ``axis`` outside ``[0, axes)`` leaves the
+    pair as it is.  Pairs are neighbours, as in :func:`rope_`, or with ``half`` elements ``j`` and ``j + head_dim/2``.  ``backward``
+    turns back."""
+    if buf.dim() != 2 or buf.dtype not in (torch.bfloat16, torch.float32) or (buf.shape[1] > 1 and buf.stride(1) != 1):
+        raise ValueError("buf must be a 2-D bf16 or fp32 tensor with unit inner stride")
+    T = buf.shape[0]
+    ld = buf.stride(0) if T > 1 else max(buf.stride(0), buf.shape[1])
+    if n_heads < 1 or head_dim < 2 or head_dim % 2 or buf.shape[1] < n_heads * head_dim or (T > 1 and ld < n_heads * head_dim):
+        raise ValueError(f"buf of shape {tuple(buf.shape)} does not hold {n_heads} heads of {head_dim}")
+    if positions.dim() != 2 or positions.shape[1] != T or positions.shape[0] < 1 or positions.dtype != torch.int32 or not positions.is_contiguous():
+        raise ValueError("positions must be contiguous int32 [axes, rows]")
+    _check_rows((("inv_freq", inv_freq, (head_dim // 2,)),), torch.float64)
+    _check_rows((("axis", axis, (head_dim // 2,)),), torch.int32)
+    _check_here((("buf", buf), ("positions", positions), ("inv_freq", inv_freq), ("axis", axis)))
+    if T == 0:
+        return buf
+    if not buf.is_cuda:
+        buf.copy_(ref_rope_axes(buf, positions, inv_freq, axis, n_heads, head_dim, half, backward))
+        return buf
+    N.check(_fn("rope_axes")(_at(buf), _at(positions), _at(inv_freq), _at(axis), T, positions.shape[0], n_heads, head_dim, ld,
+                             int(buf.dtype == torch.float32), int(half), int(backward), _stream()), "rope_axes")
     return buf
 
 
@@ -654,6 +872,155 @@ def ref_attention_lse(q, k, v, causal=True):
     return torch.logsumexp(s, dim=-1)
 
 
+class AttentionSpans:
+    """Which keys each query sees in rows of packed documents (:func:`attention_spans`): ``rows`` int32 ``[batch, seq, 4]`` holds the range
+    ``[lo, hi)`` of the keys that a token sees and the range ``[from, to)`` of the queries that see it, both empty for padding;
+    ``positions`` int32 ``[batch, seq]`` counts from 0 in every document (``positions.view(1, -1)`` goes into :func:`rope_axes_`).
+    ``tiles`` and ``padded`` are what the kernels need of 128 tokens and of a row."""
+
+    def __init__(self, batch: int, seq: int, device) -> None:
+        self.batch, self.seq, self.n_tiles = batch, seq, (seq + 127) // 128
+        sizes = (4 * batch * seq, 8 * batch * self.n_tiles, batch * seq, batch)
+        self._at = [sum(sizes[:i]) for i in range(5)]
+        self._buf = torch.empty(self._at[4], dtype=torch.int32, device=device)
+        self.device = self._buf.device
+
+    def _part(self, i: int, *shape: int) -> torch.Tensor:
+        return self._buf[self._at[i] : self._at[i + 1]].view(*shape)
+
+    @property
+    def rows(self) -> torch.Tensor:
+        return self._part(0, self.batch, self.seq, 4)
+
+    @property
+    def tiles(self) -> torch.Tensor:
+        return self._part(1, self.batch, self.n_tiles, 8)
+
+    @property
+    def positions(self) -> torch.Tensor:
+        return self._part(2, self.batch, self.seq)
+
+    @property
+    def padded(self) -> torch.Tensor:
+        return self._part(3, self.batch)
+
+    def _pointers(self) -> Tuple[int, ...]:
+        base = self._buf.data_ptr()
+        return tuple(base + 4 * a for a in self._at[:4])
+
+
+_NONE = 2**31 - 1
+
+
+def ref_attention_spans(documents, prefix=None, causal=True, window=0):
+    """``(rows, positions, tiles, padded)`` of :func:`attention_spans`."""
+    B, S = documents.shape
+    at = torch.arange(S, device=documents.device).expand(B, S)
+    first = torch.ones(B, S, dtype=torch.bool, device=documents.device)
+    first[:, 1:] = documents[:, 1:] != documents[:, :-1]
+    last = torch.ones_like(first)
+    last[:, :-1] = first[:, 1:]
+    start = torch.where(first, at, 0).cummax(1).values
+    end = torch.where(last, at + 1, S).flip(1).cummin(1).values.flip(1)
+    lo, hi, since, to = start, end, start, end
+    if causal:
+        plain = torch.where(prefix == 0, at, S) if prefix is not None else at
+        pre = torch.minimum(plain.flip(1).cummin(1).values.flip(1).gather(1, start), end)  # where a document's prefix ends
+        hi = torch.maximum(at + 1, pre)
+        since = torch.where(at < pre, start, at)
+        if window > 0:
+            lo = torch.maximum(start, at - (window - 1))
+            to = torch.minimum(end, at + window)
+    rows = torch.stack([lo, hi, since, to], -1)
+    live = (documents >= 0).unsqueeze(-1)
+    rows = torch.where(live, rows, 0)
+    n = (S + 127) // 128
+    fill = torch.zeros(B, n * 128 - S, 4, dtype=rows.dtype, device=rows.device)
+    r = torch.cat([rows, fill], 1).view(B, n, 128, 4)
+    dead, beyond = r[..., 1] <= r[..., 0], torch.arange(n * 128, device=rows.device).view(n, 128) >= S
+    least = torch.where(dead, _NONE, r[..., 0]).amin(-1), torch.where(dead, _NONE, r[..., 2]).amin(-1)
+    most = r[..., 1].amax(-1), r[..., 3].amax(-1)
+    hole = (dead & ~beyond).any(-1)
+    odd = dead.any(-1)
+    every = (torch.where(hole, _NONE, torch.where(dead, 0, r[..., 0]).amax(-1)), torch.where(hole, 0, torch.where(dead, _NONE, r[..., 1]).amin(-1)),
+             torch.where(odd, _NONE, r[..., 2].amax(-1)), torch.where(odd, 0, torch.where(dead, _NONE, r[..., 3]).amin(-1)))
+    tiles = torch.stack([least[0], most[0], every[0], every[1], least[1], most[1], every[2], every[3]], -1)
+    return rows.to(torch.int32), (at - start).to(torch.int32), tiles.to(torch.int32), (documents < 0).any(1).to(torch.int32)
+
+
+def attention_spans(documents: torch.Tensor, prefix: Optional[torch.Tensor] = None, causal: bool = True, window: int = 0) -> AttentionSpans:
+    """The mask of rows that hold documents one after another, for :func:`attention_fwd` and :func:`attention_bwd` (one for all layers and
+    both passes of a batch).  ``documents`` int32 ``[batch, seq]``: a run of equal ids is a document, whose tokens see each other only;
+    an id below zero is padding, which sees nothing (its output rows are zero) and is seen by nobody, whatever stands in it.  With
+    ``causal`` a token sees itself and those before it, at most the last ``window`` of them (itself among them) where that is not 0, and
+    the tokens that ``prefix`` (bool or uint8 ``[batch, seq]``) flags at the start of a document are seen by all of it, by each other in
+    both directions too."""
+    if documents.dim() != 2 or documents.dtype != torch.int32 or not documents.is_contiguous():
+        raise ValueError("documents must be contiguous int32 [batch, seq]")
+    if prefix is not None and (prefix.shape != documents.shape or prefix.dtype not in (torch.bool, torch.uint8) or not prefix.is_contiguous()):
+        raise ValueError("prefix must be contiguous bool or uint8 of the shape of documents")
+    if not 0 <= window < 2**31:
+        raise ValueError("window must be 0 or a number of keys")
+    if not causal and (window or prefix is not None):
+        raise ValueError("a window or a prefix goes with a causal mask")
+    _check_here((("documents", documents), ("prefix", prefix)))
+    B, S = documents.shape
+    spans = AttentionSpans(B, S, documents.device)
+    if B == 0 or S == 0:
+        return spans
+    if not documents.is_cuda:
+        for mine, t in zip((spans.rows, spans.positions, spans.tiles, spans.padded), ref_attention_spans(documents, prefix, causal, window)):
+            mine.copy_(t)
+        return spans
+    rows, tiles, positions, padded = spans._pointers()
+    N.check(_fn("attention_spans")(_at(documents), _at(prefix), rows, positions, tiles, padded, B, S, int(causal), window, _stream()),
+            "attention_spans")
+    return spans
+
+
+def ref_attention_masked(q, k, v, rows=None, causal=True, softcap=0.0, slopes=None):
+    """``(out, lse)`` of attention under a mask, in the type of the arguments: 4-D q, k, v as :func:`ref_attention`, ``rows`` as in
+    :class:`AttentionSpans`."""
+    B, S, Hq, Dh = q.shape
+    rep = Hq // k.shape[2]
+    q, k, v = q.transpose(1, 2), k.transpose(1, 2).repeat_interleave(rep, 1), v.transpose(1, 2).repeat_interleave(rep, 1)
+    s = q @ k.transpose(-1, -2) / math.sqrt(Dh)
+    if softcap > 0:
+        s = softcap * torch.tanh(s / softcap)
+    at = torch.arange(S, device=q.device)
+    if slopes is not None:
+        s = s - slopes.to(s.dtype)[:, None, None] * (at[:, None] - at[None, :]).abs()
+    if rows is not None:
+        seen = ((at >= rows[..., 0:1]) & (at < rows[..., 1:2])).unsqueeze(1)
+    else:
+        seen = (at[:, None] >= at[None, :]) | (not causal)
+    s = s.masked_fill(~seen, -math.inf)
+    top = s.detach().amax(-1, keepdim=True)
+    top = torch.where(top > -math.inf, top, 0.0)
+    p = torch.exp(s - top)
+    total = p.sum(-1, keepdim=True)
+    o = (p @ v) / torch.where(total > 0, total, 1.0)
+    return o.transpose(1, 2), (top + total.log()).squeeze(-1).detach()
+
+
+def _check_masked(named, spans: Optional[AttentionSpans], softcap: float, slopes: Optional[torch.Tensor], lse: Optional[torch.Tensor], batch: int,
+                  seq_len: int, n_heads: int, n_kv_heads: int, head_dim: int) -> None:
+    if head_dim not in (64, 128) or n_heads < 1 or n_kv_heads < 1 or n_heads % n_kv_heads:
+        raise ValueError("masked attention takes head dims 64 and 128 and groups of equally many query heads")
+    for name, t, heads in named:
+        if tuple(t.shape) != (batch * seq_len, heads * head_dim):
+            raise ValueError(f"{name} must be {(batch * seq_len, heads * head_dim)}, got {tuple(t.shape)}")
+    if not 0.0 <= softcap < math.inf:
+        raise ValueError("softcap must be 0 or a finite cap")
+    if spans is not None and (spans.batch, spans.seq) != (batch, seq_len):
+        raise ValueError(f"spans are of {(spans.batch, spans.seq)}, not of {(batch, seq_len)}")
+    if slopes is not None:
+        _check_rows((("slopes", slopes, (n_heads,)),), torch.float32)
+    if lse is not None:
+        _check_rows((("lse", lse, (batch, n_heads, seq_len)),), torch.float32)
+    _check_here([(n, t) for n, t, _ in named] + [("spans", spans), ("slopes", slopes), ("lse", lse)])
+
+
 def attention_supported(seq_len: int, head_dim: int) -> bool:
     """Shapes the tcgen05 attention kernels take: head dim 128 with 128-row blocks, or head dim 64 with
     sequences that are a multiple of 256 (the forward kernel for it works on two 128-query tiles per CTA)."""
@@ -675,14 +1042,40 @@ def _two_query_tiles(batch: int, seq_len: int, n_heads: int, sms: int) -> bool:
 
 def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: int, seq_len: int, n_heads: int,
                   n_kv_heads: int, head_dim: int, out: torch.Tensor, lse: Optional[torch.Tensor] = None,
-                  causal: bool = True, any_length: bool = False) -> None:
+                  causal: bool = True, any_length: bool = False, spans: Optional[AttentionSpans] = None, softcap: float = 0.0,
+                  slopes: Optional[torch.Tensor] = None) -> None:
     """Causal GQA attention forward.  ``q`` ``[batch*seq, n_heads*head_dim]`` and ``k``/``v``
     ``[batch*seq, n_kv_heads*head_dim]`` are 2-D bf16 views (column slices of the packed QKV
     activation are fine), ``out`` ``[batch*seq, n_heads*head_dim]``, ``lse`` ``[batch, n_heads,
     seq]`` fp32 (saved for the backward pass).  Sequence lengths are those of :func:`attention_supported`; ``any_length``
-    takes every other one as well (of head dims 64 and 128)."""
+    takes every other one as well (of head dims 64 and 128).
+
+    ``spans`` (:func:`attention_spans`) say which keys a query sees, in place of ``causal``.  ``softcap`` caps the scaled scores: ``softcap *
+    tanh(s / softcap)``; ``slopes`` (fp32 ``[n_heads]``, not differentiated) lower them by ``slope * |query - key|``.  With any of the
+    three the sequence may have any length; a row that sees nothing gets zeros and a ``lse`` of -infinity.  Keys of another document
+    that share a block of 128 with those of a row have to be finite; padding need not."""
     for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
         _check_2d_bf16(t, name)
+    if spans is not None or softcap != 0.0 or slopes is not None:
+        _check_masked((("q", q, n_heads), ("k", k, n_kv_heads), ("v", v, n_kv_heads), ("out", out, n_heads)), spans, softcap, slopes, lse, batch,
+                      seq_len, n_heads, n_kv_heads, head_dim)
+        if batch == 0 or seq_len == 0:
+            return
+        if not q.is_cuda:
+            q4, k4, v4 = (t.reshape(batch, seq_len, -1, head_dim).float() for t in (q, k, v))
+            o4, l4 = ref_attention_masked(q4, k4, v4, spans.rows if spans is not None else None, causal, softcap, slopes)
+            out.copy_(o4.reshape(batch * seq_len, -1))
+            if lse is not None:
+                lse.copy_(l4)
+            return
+        rows, tiles, _, padded = spans._pointers() if spans is not None else (None, None, None, None)
+        N.check(
+            _fn("attention_masked_fwd")(_at(q), _at(k), _at(v), _at(out), _at(lse), rows, tiles, padded, _at(slopes), batch, seq_len, n_heads,
+                                        n_kv_heads, head_dim, q.stride(0), k.stride(0), v.stride(0), out.stride(0), 1.0 / math.sqrt(head_dim),
+                                        softcap, int(causal), _status_ptr(q.device), _stream()),
+            "attention_masked_fwd",
+        )
+        return
     if not q.is_cuda:
         B, S = batch, seq_len
         q4, k4, v4 = (t.reshape(B, S, -1, head_dim) for t in (q, k, v))
@@ -738,16 +1131,36 @@ def attention_bwd_scratch_bytes(batch: int, seq_len: int, n_heads: int, n_kv_hea
 def attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, d_o: torch.Tensor,
                   lse: torch.Tensor, dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor, batch: int, seq_len: int,
                   n_heads: int, n_kv_heads: int, head_dim: int, causal: bool = True,
-                  scratch: Optional[torch.Tensor] = None, rope: Optional[torch.Tensor] = None, any_length: bool = False) -> None:
+                  scratch: Optional[torch.Tensor] = None, rope: Optional[torch.Tensor] = None, any_length: bool = False,
+                  spans: Optional[AttentionSpans] = None, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None) -> None:
     """Backward of :func:`attention_fwd`: writes ``dq``, ``dk``, ``dv`` (2-D bf16 views like
     ``q``, ``k``, ``v``; column slices of a packed dQKV buffer are fine).  The fp32 dQ
     accumulator lives in ``scratch`` (bytes on the device, :func:`attention_bwd_scratch_bytes` of
     them or more), by default a per-device buffer that is reused across calls on the same stream.
     With ``rope``, the table (:func:`rope_table`) that ``q`` and ``k`` were rotated by, ``dq`` and ``dk``
     are the gradients of the values before the rotation.  Sequences are a multiple of 128 or, with
-    ``any_length``, of any length."""
+    ``any_length``, of any length.
+
+    ``spans``, ``softcap`` and ``slopes`` as in the forward pass; with any of them sequences have any length, the default
+    ``scratch`` is this call's own, and rows that see nothing, or are seen by nobody, get zeros."""
     for t, name in ((q, "q"), (k, "k"), (v, "v"), (o, "o"), (d_o, "d_o"), (dq, "dq"), (dk, "dk"), (dv, "dv")):
         _check_2d_bf16(t, name)
+    masked = spans is not None or softcap != 0.0 or slopes is not None
+    if masked:
+        _check_masked((("q", q, n_heads), ("k", k, n_kv_heads), ("v", v, n_kv_heads), ("o", o, n_heads), ("d_o", d_o, n_heads), ("dq", dq, n_heads),
+                       ("dk", dk, n_kv_heads), ("dv", dv, n_kv_heads)), spans, softcap, slopes, lse, batch, seq_len, n_heads, n_kv_heads, head_dim)
+        if batch == 0 or seq_len == 0:
+            return
+        if not q.is_cuda:
+            q4, k4, v4 = (t.detach().reshape(batch, seq_len, -1, head_dim).float().requires_grad_(True) for t in (q, k, v))
+            with torch.enable_grad():
+                o4, _ = ref_attention_masked(q4, k4, v4, spans.rows if spans is not None else None, causal, softcap, slopes)
+            for to, g in zip((dq, dk, dv), torch.autograd.grad(o4, (q4, k4, v4), d_o.reshape(batch, seq_len, -1, head_dim).float())):
+                to.copy_(g.reshape(batch * seq_len, -1))
+            if rope is not None:
+                dq.copy_(ref_rope(dq, rope, seq_len, n_heads, head_dim, backward=True))
+                dk.copy_(ref_rope(dk, rope, seq_len, n_kv_heads, head_dim, backward=True))
+            return
     if not q.is_cuda:
         B, S = batch, seq_len
         q4, k4, v4, do4 = (t.reshape(B, S, -1, head_dim) for t in (q, k, v, d_o))
@@ -759,14 +1172,15 @@ def attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Te
             dq.copy_(ref_rope(dq, rope, S, n_heads, head_dim, backward=True))
             dk.copy_(ref_rope(dk, rope, S, n_kv_heads, head_dim, backward=True))
         return
-    if seq_len % 128 and not any_length:
+    if seq_len % 128 and not (any_length or masked):
         N.check(-1, "attention_bwd")
     if rope is not None and (rope.dtype != torch.float32 or not rope.is_contiguous() or rope.device != q.device
                              or rope.shape[0] < seq_len or tuple(rope.shape[1:]) != (head_dim // 2, 2)):
         raise ValueError("rope must be the table of the sequence and head dim on the device of q")
-    lib = N.lib()
     need = attention_bwd_scratch_bytes(batch, seq_len, n_heads, n_kv_heads)
-    if scratch is None:
+    if scratch is None and masked:
+        scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+    elif scratch is None:
         key = (q.device.index, _stream())
         scratch = _attn_scratch.get(key)
         if scratch is None or scratch.numel() < need:
@@ -775,6 +1189,16 @@ def attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Te
     elif scratch.device != q.device or scratch.dtype != torch.uint8 or scratch.numel() < need or not scratch.is_contiguous():
         raise ValueError(f"scratch must be {need} contiguous bytes on {q.device}")
     scale = 1.0 / math.sqrt(head_dim)
+    if masked:
+        rows, tiles, _, padded = spans._pointers() if spans is not None else (None, None, None, None)
+        N.check(
+            _fn("attention_masked_bwd")(_at(q), _at(k), _at(v), _at(o), _at(d_o), _at(lse), _at(dq), _at(dk), _at(dv), _at(scratch), rows, tiles,
+                                        padded, _at(slopes), batch, seq_len, n_heads, n_kv_heads, head_dim, q.stride(0), k.stride(0), v.stride(0),
+                                        o.stride(0), d_o.stride(0), dq.stride(0), dk.stride(0), dv.stride(0), scale, softcap, int(causal),
+                                        _at(rope), _status_ptr(q.device), _stream()),
+            "attention_masked_bwd", launches=3,
+        )
+        return
     N.check(
         _fn("attention_bwd")(_at(q), _at(k), _at(v), _at(o), _at(d_o), _at(lse), _at(dq), _at(dk), _at(dv), _at(scratch),
                              batch, seq_len, n_heads, n_kv_heads, head_dim, q.stride(0), k.stride(0), v.stride(0), o.stride(0),
