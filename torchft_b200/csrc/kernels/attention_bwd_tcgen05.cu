@@ -161,7 +161,7 @@ template <int D, bool MASK, bool SCORE>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
-                     const BwdParams p) {
+                     const __grid_constant__ CUtensorMap tmDK, const __grid_constant__ CUtensorMap tmDV, const BwdParams p) {
   using Ly = Lay<D>;
   constexpr int SLABS = Ly::SLABS;
   constexpr uint32_t TILE = Ly::TILE;
@@ -606,9 +606,6 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       for (int which = 0; which < 2; ++which) {
         constexpr int CW = D / 2;  // head-dim columns per thread
         const uint32_t col = (which == 0 ? Ly::COL_DV : Ly::COL_DK) + g * CW;
-        __nv_bfloat16* base = which == 0 ? p.dV : p.dK;
-        const long long ld = which == 0 ? p.ld_dv : p.ld_dk;
-        __nv_bfloat16* dst = base + (static_cast<long long>(b) * p.seq + jb * BKV + row) * ld + hk * D + g * CW;
         uint32_t v[CW];
 #pragma unroll
         for (int c = 0; c < CW / 32; ++c) tmem_ld32(tmem_base + col + c * 32 + lane_addr, v + c * 32);
@@ -626,19 +623,32 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                                         __uint_as_float(v[4 * c + 3]));
           continue;
         }
+        // They leave by TMA, 32 keys of CW elements a warp, from where K and V were, whose last product is done.
+        const uint32_t off = (which == 0 ? Ly::OFF_V : Ly::OFF_K) + (warp - 8) * (32 * CW * 2);
+        uint8_t* stage = smem + off + lane * (CW * 2);
+        const int swizzle = CW == 64 ? lane & 7 : lane >> 1 & 3;  // 128 or 64 bytes wide
 #pragma unroll
         for (int c = 0; c < CW / 8; ++c) {
           float f[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(v[8 * c + e]);
-          if (beyond) continue;
-          if (which == 1 && p.rope != nullptr) {
+          if (which == 1 && p.rope != nullptr && !beyond) {
             const float4* cs = p.rope + static_cast<long long>(jb * BKV + row) * (D / 4) + g * (CW / 4) + 2 * c;
             rotate_back(f, cs[0], cs[1]);
           }
-          reinterpret_cast<ftb200::bf16x8*>(dst)[c] = ftb200::pack8(f);
+          *reinterpret_cast<ftb200::bf16x8*>(stage + ((c ^ swizzle) << 4)) = ftb200::pack8(f);
         }
+        fence_async_smem();
+        __syncwarp();
+        const int first = jb * BKV + quarter * 32;
+        if (first < p.seq && elect_one()) {
+          tma_store_3d(which == 0 ? &tmDV : &tmDK, smem_base + off, hk * D + g * CW, first, b);
+          bulk_commit();
+        }
+        __syncwarp();
       }
+      // the shared memory has been read; elect_one may take another lane, so all wait for what they have committed
+      bulk_wait_read();
     }
   }
 
@@ -823,16 +833,19 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// [batch, seq, cols] bf16 view with row stride ld (elements); box = 64 columns x 128 rows, 128-byte swizzle
-int encode_rows(CUtensorMap* map, const void* base, long long batch, long long seq, long long cols, long long ld) {
+// [batch, seq, cols] bf16 view with row stride ld (elements); box = 64 columns x 128 rows, 128-byte swizzle (dK, dV: half a head x 32 rows, the
+// swizzle as wide as the box)
+int encode_rows(CUtensorMap* map, const void* base, long long batch, long long seq, long long cols, long long ld, unsigned box_cols = 64,
+                unsigned box_rows = 128) {
   auto fn = encode_fn();
   if (fn == nullptr) return FTB200_E_DRIVER;
   cuuint64_t gdim[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(seq), static_cast<cuuint64_t>(batch)};
   cuuint64_t gstride[2] = {static_cast<cuuint64_t>(ld) * 2, static_cast<cuuint64_t>(seq) * ld * 2};
-  cuuint32_t box[3] = {64u, 128u, 1u};
+  cuuint32_t box[3] = {box_cols, box_rows, 1u};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), gdim, gstride, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : FTB200_E_DRIVER;
 }
@@ -868,11 +881,13 @@ int attention_bwd_impl(const void* q, const void* k, const void* v, const void* 
   float* neg_lse2 = neg_delta + rows * n_heads;
   const int split = head_split(batch * tiles * n_kv_heads, n_heads / n_kv_heads);
   if (rows > 0x7fffffffLL) return FTB200_E_TOOBIG;
-  CUtensorMap tq, tk, tv, tdo;
+  CUtensorMap tq, tk, tv, tdo, tdk, tdv;
   int rc = encode_rows(&tq, q, batch, seq, static_cast<long long>(n_heads) * D, ld_q);
   if (rc == 0) rc = encode_rows(&tdo, d_o, batch, seq, static_cast<long long>(n_heads) * D, ld_do);
   if (rc == 0) rc = encode_rows(&tk, k, batch, seq, static_cast<long long>(n_kv_heads) * D, ld_k);
   if (rc == 0) rc = encode_rows(&tv, v, batch, seq, static_cast<long long>(n_kv_heads) * D, ld_v);
+  if (rc == 0) rc = encode_rows(&tdk, dk, batch, seq, static_cast<long long>(n_kv_heads) * D, ld_dk, D / 2, 32);
+  if (rc == 0) rc = encode_rows(&tdv, dv, batch, seq, static_cast<long long>(n_kv_heads) * D, ld_dv, D / 2, 32);
   if (rc != 0) return rc;
   static bool attr_set = false;
   if (!attr_set) {
@@ -901,8 +916,8 @@ int attention_bwd_impl(const void* q, const void* k, const void* v, const void* 
   p.dkv_part = reinterpret_cast<float4*>(neg_lse2 + rows * n_heads);
   const long long grid = static_cast<long long>(batch) * n_kv_heads * tiles * split;
   if (grid > 0x7fffffffLL) return FTB200_E_TOOBIG;
-  ftb200::launch_after(kernel, static_cast<unsigned>(grid), NUM_THREADS, SMEM_BYTES, stream, tq, tk, tv, tdo,
-      p);
+  ftb200::launch_after(kernel, static_cast<unsigned>(grid), NUM_THREADS, SMEM_BYTES, stream, tq, tk, tv, tdo, tdk,
+      tdv, p);
   const long long cast_warps = batch * tiles * n_heads * (D / 64) * (32 / CAST_GROUPS);
   const long long dkv_blocks = split > 1 ? static_cast<long long>(batch) * n_kv_heads * tiles * (2 * D / 32) : 0;
   const long long cast_blocks = dkv_blocks + (cast_warps + 7) / 8;  // fewer than the first kernel's

@@ -81,8 +81,6 @@ struct Attn2Params {
   int batch, seq, n_heads, n_kv_heads;
   int causal;
   float scale_log2;  // softmax scale * log2(e)
-  __nv_bfloat16* O;
-  long long ld_o;    // row stride of O in elements
   float* lse;        // [batch, n_heads, seq], natural log
   int* status;
   ftb200::MaskParams mask;  // of the kernels with MASK
@@ -105,7 +103,7 @@ enum : int {
 template <int D, int POLY, bool MASK, bool SCORE>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 attention_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                      const __grid_constant__ CUtensorMap tmV, const Attn2Params p) {
+                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const Attn2Params p) {
   using C = Cfg<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -472,8 +470,9 @@ attention_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
       tc_fence_after();
       const bool nothing = MASK && l_sum == 0.f;  // no key is seen: zeros, and a log-sum-exp of -infinity
       const float inv = 1.f / l_sum;
-      const bool stored = query < p.seq;
-      __nv_bfloat16* dst = p.O + (static_cast<long long>(b) * p.seq + query) * p.ld_o + head * D;
+      // O leaves by TMA, 32 rows a warp, from the place of this tile's Q, whose last product is done.  Stored by the threads, 16 bytes of 32 rows an
+      // instruction, it held every CTA up for 9.2 us.
+      uint8_t* stage = smem + C::OFF_Q + t * C::TILE_BYTES + row * 128;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t ov[32];
@@ -484,10 +483,20 @@ attention_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
           float f[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) f[e] = nothing ? 0.f : __uint_as_float(ov[8 * q4 + e]) * inv;
-          if (stored) reinterpret_cast<ftb200::bf16x8*>(dst + c * 32)[q4] = ftb200::pack8(f);
+          *reinterpret_cast<ftb200::bf16x8*>(stage + (c >> 1) * C::SLAB_BYTES + ((((c & 1) * 4 + q4) ^ (row & 7)) << 4)) = ftb200::pack8(f);
         }
       }
-      if (p.lse != nullptr && stored) {
+      fence_async_smem();
+      __syncwarp();
+      const int first = q0 + t * q_step + quarter * 32;
+      if (first < p.seq && elect_one()) {
+        for (int s = 0; s < C::SLABS; ++s)
+          tma_store_3d(&tmO, smem_base + C::OFF_Q + t * C::TILE_BYTES + s * C::SLAB_BYTES + quarter * (32 * 128), head * D + s * 64, first, b);
+        bulk_commit();
+        bulk_wait_read();
+      }
+      __syncwarp();
+      if (p.lse != nullptr && query < p.seq) {
         p.lse[(static_cast<long long>(b) * p.n_heads + head) * p.seq + query] =
             nothing ? -INFINITY : (m_used * scale_log2 + log2f(l_sum)) * 0.6931471805599453f;
       }
@@ -518,13 +527,13 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn2() {
   return fn;
 }
 
-// [batch, seq, cols] bf16 view with row stride ld (elements); box = 64 columns x 128 rows, 128-byte swizzle
-int encode_rows2(CUtensorMap* map, const void* base, long long batch, long long seq, long long cols, long long ld) {
+// [batch, seq, cols] bf16 view with row stride ld (elements); box = 64 columns x 128 rows (O: 32), 128-byte swizzle
+int encode_rows2(CUtensorMap* map, const void* base, long long batch, long long seq, long long cols, long long ld, unsigned box_rows = 128) {
   auto fn = encode_fn2();
   if (fn == nullptr) return FTB200_E_DRIVER;
   cuuint64_t gdim[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(seq), static_cast<cuuint64_t>(batch)};
   cuuint64_t gstride[2] = {static_cast<cuuint64_t>(ld) * 2, static_cast<cuuint64_t>(seq) * ld * 2};
-  cuuint32_t box[3] = {64u, 128u, 1u};
+  cuuint32_t box[3] = {64u, box_rows, 1u};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), gdim, gstride, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -532,9 +541,12 @@ int encode_rows2(CUtensorMap* map, const void* base, long long batch, long long 
   return r == CUDA_SUCCESS ? 0 : FTB200_E_DRIVER;
 }
 
+struct Maps {
+  CUtensorMap q, k, v, o;
+};
+
 template <int D, int POLY, bool MASK = false, bool SCORE = false>
-int launch_fwd2(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const Attn2Params& p, long long grid,
-                cudaStream_t stream) {
+int launch_fwd2(const Maps& m, const Attn2Params& p, long long grid, cudaStream_t stream) {
   auto* kernel = attention_fwd2_kernel<D, POLY, MASK, SCORE>;
   static bool attr_set = false;
   if (!attr_set) {
@@ -547,21 +559,22 @@ int launch_fwd2(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap&
     if (attr.numRegs < LAUNCH_REGS) return FTB200_E_REGS;
     attr_set = true;
   }
-  ftb200::launch_after(kernel, static_cast<unsigned>(grid), NUM_THREADS, Cfg<D>::SMEM_BYTES, stream, tq, tk, tv, p);
+  ftb200::launch_after(kernel, static_cast<unsigned>(grid), NUM_THREADS, Cfg<D>::SMEM_BYTES, stream, m.q, m.k, m.v, m.o, p);
   return cudaGetLastError() == cudaSuccess ? 0 : FTB200_E_CUDA;
 }
 
-int make_maps(CUtensorMap* tq, CUtensorMap* tk, CUtensorMap* tv, const void* q, const void* k, const void* v, const void* o, int batch, int seq,
-              int n_heads, int n_kv_heads, int head_dim, long long ld_q, long long ld_k, long long ld_v, long long ld_o) {
+int make_maps(Maps* m, const void* q, const void* k, const void* v, const void* o, int batch, int seq, int n_heads, int n_kv_heads, int head_dim,
+              long long ld_q, long long ld_k, long long ld_v, long long ld_o) {
   if ((head_dim != 64 && head_dim != 128) || batch <= 0 || seq <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0)
     return FTB200_E_BADARG;
   auto aligned16 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || (ld_q & 7) || (ld_k & 7) || (ld_v & 7) ||
       (ld_o & 7))
     return FTB200_E_ALIGN;
-  int rc = encode_rows2(tq, q, batch, seq, static_cast<long long>(n_heads) * head_dim, ld_q);
-  if (rc == 0) rc = encode_rows2(tk, k, batch, seq, static_cast<long long>(n_kv_heads) * head_dim, ld_k);
-  if (rc == 0) rc = encode_rows2(tv, v, batch, seq, static_cast<long long>(n_kv_heads) * head_dim, ld_v);
+  int rc = encode_rows2(&m->q, q, batch, seq, static_cast<long long>(n_heads) * head_dim, ld_q);
+  if (rc == 0) rc = encode_rows2(&m->k, k, batch, seq, static_cast<long long>(n_kv_heads) * head_dim, ld_k);
+  if (rc == 0) rc = encode_rows2(&m->v, v, batch, seq, static_cast<long long>(n_kv_heads) * head_dim, ld_v);
+  if (rc == 0) rc = encode_rows2(&m->o, o, batch, seq, static_cast<long long>(n_heads) * head_dim, ld_o, 32);
   return rc;
 }
 
@@ -576,23 +589,23 @@ FTB200_API int ftb200_attention_fwd2(const void* q, const void* k, const void* v
                                      long long ld_v, long long ld_o, float scale, int causal, int poly, int* status,
                                      cudaStream_t stream) {
   if (poly != 0 && poly != 2 && poly != 4) return FTB200_E_BADARG;
-  CUtensorMap tq, tk, tv;
-  const int rc = make_maps(&tq, &tk, &tv, q, k, v, o, batch, seq, n_heads, n_kv_heads, head_dim, ld_q, ld_k, ld_v, ld_o);
+  Maps m;
+  const int rc = make_maps(&m, q, k, v, o, batch, seq, n_heads, n_kv_heads, head_dim, ld_q, ld_k, ld_v, ld_o);
   if (rc != 0) return rc;
   Attn2Params p = {};
   p.batch = batch; p.seq = seq; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads; p.causal = causal;
   p.scale_log2 = scale * 1.4426950408889634f;
-  p.O = reinterpret_cast<__nv_bfloat16*>(o); p.ld_o = ld_o; p.lse = lse; p.status = status;
+  p.lse = lse; p.status = status;
   const long long grid = static_cast<long long>(batch) * n_heads * ((static_cast<long long>(seq) + BQ * TILES - 1) / (BQ * TILES));
   if (grid > 0x7fffffffLL) return FTB200_E_TOOBIG;
   if (head_dim == 128) {
-    if (poly == 0) return launch_fwd2<128, 0>(tq, tk, tv, p, grid, stream);
-    if (poly == 2) return launch_fwd2<128, 2>(tq, tk, tv, p, grid, stream);
-    return launch_fwd2<128, 4>(tq, tk, tv, p, grid, stream);
+    if (poly == 0) return launch_fwd2<128, 0>(m, p, grid, stream);
+    if (poly == 2) return launch_fwd2<128, 2>(m, p, grid, stream);
+    return launch_fwd2<128, 4>(m, p, grid, stream);
   }
-  if (poly == 0) return launch_fwd2<64, 0>(tq, tk, tv, p, grid, stream);
-  if (poly == 2) return launch_fwd2<64, 2>(tq, tk, tv, p, grid, stream);
-  return launch_fwd2<64, 4>(tq, tk, tv, p, grid, stream);
+  if (poly == 0) return launch_fwd2<64, 0>(m, p, grid, stream);
+  if (poly == 2) return launch_fwd2<64, 2>(m, p, grid, stream);
+  return launch_fwd2<64, 4>(m, p, grid, stream);
 }
 
 // The same under a mask (attention_masks.cuh).  rows, tiles, padded: null, where every query sees the keys up to its own (causal) or all, or what
@@ -602,14 +615,14 @@ FTB200_API int ftb200_attention_masked_fwd(const void* q, const void* k, const v
                                            const int* padded, const float* slopes, int batch, int seq, int n_heads, int n_kv_heads, int head_dim,
                                            long long ld_q, long long ld_k, long long ld_v, long long ld_o, float scale, float softcap, int causal,
                                            int* status, cudaStream_t stream) {
-  CUtensorMap tq, tk, tv;
-  int rc = make_maps(&tq, &tk, &tv, q, k, v, o, batch, seq, n_heads, n_kv_heads, head_dim, ld_q, ld_k, ld_v, ld_o);
+  Maps m;
+  int rc = make_maps(&m, q, k, v, o, batch, seq, n_heads, n_kv_heads, head_dim, ld_q, ld_k, ld_v, ld_o);
   Attn2Params p = {};
   if (rc == 0) rc = ftb200::set_mask(&p.mask, rows, tiles, padded, slopes, scale, softcap, causal, seq);
   if (rc != 0) return rc;
   p.batch = batch; p.seq = seq; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads; p.causal = causal;
   p.scale_log2 = scale * 1.4426950408889634f;
-  p.O = reinterpret_cast<__nv_bfloat16*>(o); p.ld_o = ld_o; p.lse = lse; p.status = status;
+  p.lse = lse; p.status = status;
   p.pair_heads = n_heads / n_kv_heads % TILES == 0;
   const long long tiles_q = (static_cast<long long>(seq) + BQ - 1) / BQ;
   const long long grid = p.pair_heads ? batch * (static_cast<long long>(n_heads) / TILES) * tiles_q
@@ -617,6 +630,6 @@ FTB200_API int ftb200_attention_masked_fwd(const void* q, const void* k, const v
   if (grid > 0x7fffffffLL) return FTB200_E_TOOBIG;
   const bool score = softcap > 0.f || slopes != nullptr;
   if (head_dim == 128)
-    return score ? launch_fwd2<128, 0, true, true>(tq, tk, tv, p, grid, stream) : launch_fwd2<128, 0, true, false>(tq, tk, tv, p, grid, stream);
-  return score ? launch_fwd2<64, 0, true, true>(tq, tk, tv, p, grid, stream) : launch_fwd2<64, 2, true, false>(tq, tk, tv, p, grid, stream);
+    return score ? launch_fwd2<128, 0, true, true>(m, p, grid, stream) : launch_fwd2<128, 0, true, false>(m, p, grid, stream);
+  return score ? launch_fwd2<64, 0, true, true>(m, p, grid, stream) : launch_fwd2<64, 2, true, false>(m, p, grid, stream);
 }
