@@ -54,7 +54,7 @@ def test_spans_are_the_definition_s(causal, prefix, window, seed):
     live = ids[0] >= 0
     for c in range(4):  # what the kernels' ranges of tiles rest on
         assert (rows[live, c].diff() >= 0).all()
-    assert spans.padded.tolist() == [1] and spans.tiles.shape == (1, 1, 8)
+    assert spans.padded.tolist() == [[1]] and spans.tiles.shape == (1, 1, 8)
     assert spans.positions[0, 0] == 0 and (spans.positions[0][1:] - spans.positions[0][:-1] <= 1).all()
 
 

@@ -344,7 +344,7 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       };
       // S^T of the next tile is issued ahead of the products that wait for this tile's dS^T, so that its softmax runs
       // under them; the columns of S^T are free for it as P^T's reader, dV, was issued before.
-      const bool padded = MASK && p.mask.has_padding(b);
+      const bool padded = MASK && p.mask.has_padding(b, p.seq, lane);
       TileWalk next{h0, first_q};  // the tile whose Q or dO is waited for
       auto clear = [&](uint32_t off, int tile) {
         if (padded) p.mask.clear_padding(smem + off, SLABS, b, tile, p.seq, lane);

@@ -257,7 +257,7 @@ attention_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         }
         __syncwarp();
       };
-      const bool padded = MASK && p.mask.has_padding(b);
+      const bool padded = MASK && p.mask.has_padding(b, p.seq, lane);
       bool ok = n_kv1 > 0 && mbar_wait_warp(bar(BAR_Q_FULL + 0), 0, abort_flag) && mbar_wait_warp(bar(BAR_K_FULL + 0), 0, abort_flag);
       // what stands in padding reaches neither the products nor the choice of a way for the scores
       auto clear = [&](uint32_t off, int tile) {

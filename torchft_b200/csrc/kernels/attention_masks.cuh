@@ -42,7 +42,7 @@ struct RowMask {
 struct MaskParams {
   const int4* rows;  // null, or [batch][seq]: lo, hi, from, to
   const int4* tiles;  // [batch][tiles of 128][2]: (lo, hi, all_lo, all_hi), (from, to, all_from, all_to)
-  const int* padded;  // [batch]: whether a row has padding
+  const int* padded;  // [batch][blocks of 1024]: whether there is padding
   int causal;         // without rows
   int capped;
   const float* slopes;  // null, or [heads]
@@ -107,7 +107,14 @@ struct MaskParams {
     return {r.z, r.w, x.z, x.w};
   }
 
-  __device__ __forceinline__ bool has_padding(int b) const { return rows != nullptr && padded[b] != 0; }
+  // By a whole warp: whether there is padding in the sequence.
+  __device__ __forceinline__ bool has_padding(int b, int seq, int lane) const {
+    if (rows == nullptr) return false;
+    const int n = (seq + 1023) / 1024;
+    int any = 0;
+    for (int i = lane; i < n; i += 32) any |= padded[static_cast<long long>(b) * n + i];
+    return __any_sync(0xffffffffu, any);
+  }
 
   // Rows of a tile in shared memory (slabs of 128 rows x 128 bytes) that belong to padding become zeros, by one warp: what stands in padding may
   // be anything, and zero times infinity would reach the tile's other rows.  The products that follow see it.

@@ -387,20 +387,19 @@ def rmsnorm_bwd(
 # --------------------------------------------------------------------------- layer norm
 
 
-def _check_here(named) -> None:
-    """The tensors are on the current device, whose stream the kernel is launched on."""
-    device = next(t for _, t in named if t is not None).device
-    for name, t in named:
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, not on {device}")
-    if device.type == "cuda" and device.index != torch._C._cuda_getDevice():
-        raise ValueError(f"the tensors are on {device}, which is not the current device")
+def _check_here(first: torch.Tensor) -> None:
+    """The tensors' device (``first`` is one of them) is the current one, on whose stream the kernel is launched."""
+    if first.is_cuda and first.get_device() != torch._C._cuda_getDevice():
+        raise ValueError(f"the tensors are on {first.device}, which is not the current device")
 
 
-def _check_rows(named, dtype: torch.dtype) -> None:
-    for name, t, shape in named:
-        if t is not None and (t.dtype != dtype or t.shape != shape or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous {dtype} of shape {tuple(shape)}, got {t.dtype} of {tuple(t.shape)}")
+def _check_like(names: str, dtype: torch.dtype, shape, device: int, *tensors: Optional[torch.Tensor]) -> None:
+    """Each of ``tensors`` that is not None is contiguous, of the type and shape, and on the device (-1: the CPU)."""
+    for i, t in enumerate(tensors):
+        if t is not None and (t.dtype != dtype or t.shape != shape or t.get_device() != device or t.is_meta or not t.is_contiguous()):
+            where = "the CPU" if device < 0 else f"cuda:{device}"
+            raise ValueError(f"{names.split()[i]} must be contiguous {dtype} of shape {tuple(shape)} on {where}, got {t.dtype} of {tuple(t.shape)} "
+                             f"on {t.device}")
 
 
 def _check_norm(x: torch.Tensor) -> None:
@@ -443,10 +442,11 @@ def layernorm_fwd(
         h_out = torch.empty_like(x)
     if out is None:
         out = torch.empty_like(x)
-    _check_rows((("x", x, x.shape), ("w", w, (D,)), ("b", b, (D,)), ("res", res, x.shape), ("h_out", h_out, x.shape), ("out", out, x.shape)),
-                x.dtype)
-    _check_rows((("mean", mean, (T,)), ("rstd", rstd, (T,))), torch.float32)
-    _check_here((("x", x), ("w", w), ("b", b), ("res", res), ("h_out", h_out), ("out", out), ("mean", mean), ("rstd", rstd)))
+    _check_here(x)
+    dtype, at = x.dtype, x.get_device()
+    _check_like("x res h_out out", dtype, x.shape, at, x, res, h_out, out)
+    _check_like("w b", dtype, (D,), at, w, b)
+    _check_like("mean rstd", torch.float32, (T,), at, mean, rstd)
     if out is h_out and res is not None:
         raise ValueError("out and h_out are two results")
     if T > 0:
@@ -511,11 +511,11 @@ def layernorm_bwd(
         db = None
     elif db is None:
         db = torch.empty_like(w)
-    _check_rows((("x", x, x.shape), ("dy", dy, x.shape), ("w", w, (D,)), ("dres", dres, x.shape), ("dx", dx, x.shape), ("dw", dw, (D,)),
-                 ("db", db, (D,))), x.dtype)
-    _check_rows((("mean", mean, (T,)), ("rstd", rstd, (T,))), torch.float32)
-    _check_here((("x", x), ("dy", dy), ("w", w), ("mean", mean), ("rstd", rstd), ("dres", dres), ("dx", dx), ("dw", dw), ("db", db),
-                 ("scratch", scratch)))
+    _check_here(x)
+    dtype, at = x.dtype, x.get_device()
+    _check_like("x dy dres dx", dtype, x.shape, at, x, dy, dres, dx)
+    _check_like("w dw db", dtype, (D,), at, w, dw, db)
+    _check_like("mean rstd", torch.float32, (T,), at, mean, rstd)
     if T == 0:
         if not accumulate:
             dw.zero_()
@@ -532,7 +532,8 @@ def layernorm_bwd(
     need = layernorm_bwd_scratch_floats(D)
     if scratch is None:
         scratch = torch.empty(need, dtype=torch.float32, device=x.device)
-    elif scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < need or scratch.data_ptr() % 16:
+    elif (scratch.device != x.device or scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < need
+          or scratch.data_ptr() % 16):
         raise ValueError(f"scratch must be {need} contiguous fp32 on {x.device}")
     N.check(_fn("layernorm_bwd")(_at(dy), _at(x), _at(w), _at(mean), _at(rstd), _at(dres), _at(dx), _at(dw), _at(db), _at(scratch), T, D,
                                  int(accumulate), int(x.dtype == torch.float32), _stream()), "layernorm_bwd", launches=2)
@@ -623,11 +624,13 @@ def rope_axes_(buf: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tenso
     ld = buf.stride(0) if T > 1 else max(buf.stride(0), buf.shape[1])
     if n_heads < 1 or head_dim < 2 or head_dim % 2 or buf.shape[1] < n_heads * head_dim or (T > 1 and ld < n_heads * head_dim):
         raise ValueError(f"buf of shape {tuple(buf.shape)} does not hold {n_heads} heads of {head_dim}")
-    if positions.dim() != 2 or positions.shape[1] != T or positions.shape[0] < 1 or positions.dtype != torch.int32 or not positions.is_contiguous():
+    if positions.dim() != 2 or positions.shape[0] < 1:
         raise ValueError("positions must be contiguous int32 [axes, rows]")
-    _check_rows((("inv_freq", inv_freq, (head_dim // 2,)),), torch.float64)
-    _check_rows((("axis", axis, (head_dim // 2,)),), torch.int32)
-    _check_here((("buf", buf), ("positions", positions), ("inv_freq", inv_freq), ("axis", axis)))
+    _check_here(buf)
+    at = buf.get_device()
+    _check_like("positions", torch.int32, (positions.shape[0], T), at, positions)
+    _check_like("inv_freq", torch.float64, (head_dim // 2,), at, inv_freq)
+    _check_like("axis", torch.int32, (head_dim // 2,), at, axis)
     if T == 0:
         return buf
     if not buf.is_cuda:
@@ -876,14 +879,22 @@ class AttentionSpans:
     """Which keys each query sees in rows of packed documents (:func:`attention_spans`): ``rows`` int32 ``[batch, seq, 4]`` holds the range
     ``[lo, hi)`` of the keys that a token sees and the range ``[from, to)`` of the queries that see it, both empty for padding;
     ``positions`` int32 ``[batch, seq]`` counts from 0 in every document (``positions.view(1, -1)`` goes into :func:`rope_axes_`).
-    ``tiles`` and ``padded`` are what the kernels need of 128 tokens and of a row."""
+    ``tiles`` and ``padded`` are what the kernels need of 128 and of 1024 tokens."""
 
     def __init__(self, batch: int, seq: int, device) -> None:
         self.batch, self.seq, self.n_tiles = batch, seq, (seq + 127) // 128
-        sizes = (4 * batch * seq, 8 * batch * self.n_tiles, batch * seq, batch)
-        self._at = [sum(sizes[:i]) for i in range(5)]
+        a = 4 * batch * seq
+        b = a + 8 * batch * self.n_tiles
+        c = b + batch * seq
+        self._at = (0, a, b, c, c + batch * ((seq + 1023) // 1024))
         self._buf = torch.empty(self._at[4], dtype=torch.int32, device=device)
-        self.device = self._buf.device
+
+    @property
+    def device(self) -> torch.device:
+        return self._buf.device
+
+    def get_device(self) -> int:
+        return self._buf.get_device()
 
     def _part(self, i: int, *shape: int) -> torch.Tensor:
         return self._buf[self._at[i] : self._at[i + 1]].view(*shape)
@@ -902,11 +913,12 @@ class AttentionSpans:
 
     @property
     def padded(self) -> torch.Tensor:
-        return self._part(3, self.batch)
+        return self._part(3, self.batch, (self.seq + 1023) // 1024)
 
-    def _pointers(self) -> Tuple[int, ...]:
+    def _pointers(self) -> Tuple[int, int, int, int]:
         base = self._buf.data_ptr()
-        return tuple(base + 4 * a for a in self._at[:4])
+        _, a, b, c, _ = self._at
+        return base, base + 4 * a, base + 4 * b, base + 4 * c
 
 
 _NONE = 2**31 - 1
@@ -945,7 +957,8 @@ def ref_attention_spans(documents, prefix=None, causal=True, window=0):
     every = (torch.where(hole, _NONE, torch.where(dead, 0, r[..., 0]).amax(-1)), torch.where(hole, 0, torch.where(dead, _NONE, r[..., 1]).amin(-1)),
              torch.where(odd, _NONE, r[..., 2].amax(-1)), torch.where(odd, 0, torch.where(dead, _NONE, r[..., 3]).amin(-1)))
     tiles = torch.stack([least[0], most[0], every[0], every[1], least[1], most[1], every[2], every[3]], -1)
-    return rows.to(torch.int32), (at - start).to(torch.int32), tiles.to(torch.int32), (documents < 0).any(1).to(torch.int32)
+    return rows.to(torch.int32), (at - start).to(torch.int32), tiles.to(torch.int32), torch.stack(
+        [(documents[:, i : i + 1024] < 0).any(1) for i in range(0, S, 1024)], 1).to(torch.int32)
 
 
 def attention_spans(documents: torch.Tensor, prefix: Optional[torch.Tensor] = None, causal: bool = True, window: int = 0) -> AttentionSpans:
@@ -957,13 +970,15 @@ def attention_spans(documents: torch.Tensor, prefix: Optional[torch.Tensor] = No
     both directions too."""
     if documents.dim() != 2 or documents.dtype != torch.int32 or not documents.is_contiguous():
         raise ValueError("documents must be contiguous int32 [batch, seq]")
-    if prefix is not None and (prefix.shape != documents.shape or prefix.dtype not in (torch.bool, torch.uint8) or not prefix.is_contiguous()):
-        raise ValueError("prefix must be contiguous bool or uint8 of the shape of documents")
+    if prefix is not None:
+        if prefix.dtype not in (torch.bool, torch.uint8):
+            raise ValueError("prefix must be bool or uint8")
+        _check_like("prefix", prefix.dtype, documents.shape, documents.get_device(), prefix)
     if not 0 <= window < 2**31:
         raise ValueError("window must be 0 or a number of keys")
     if not causal and (window or prefix is not None):
         raise ValueError("a window or a prefix goes with a causal mask")
-    _check_here((("documents", documents), ("prefix", prefix)))
+    _check_here(documents)
     B, S = documents.shape
     spans = AttentionSpans(B, S, documents.device)
     if B == 0 or S == 0:
@@ -1003,22 +1018,28 @@ def ref_attention_masked(q, k, v, rows=None, causal=True, softcap=0.0, slopes=No
     return o.transpose(1, 2), (top + total.log()).squeeze(-1).detach()
 
 
-def _check_masked(named, spans: Optional[AttentionSpans], softcap: float, slopes: Optional[torch.Tensor], lse: Optional[torch.Tensor], batch: int,
-                  seq_len: int, n_heads: int, n_kv_heads: int, head_dim: int) -> None:
+def _check_masked(of_q, of_kv, spans: Optional[AttentionSpans], softcap: float, slopes: Optional[torch.Tensor], lse: Optional[torch.Tensor],
+                  batch: int, seq_len: int, n_heads: int, n_kv_heads: int, head_dim: int) -> None:
     if head_dim not in (64, 128) or n_heads < 1 or n_kv_heads < 1 or n_heads % n_kv_heads:
         raise ValueError("masked attention takes head dims 64 and 128 and groups of equally many query heads")
-    for name, t, heads in named:
-        if tuple(t.shape) != (batch * seq_len, heads * head_dim):
-            raise ValueError(f"{name} must be {(batch * seq_len, heads * head_dim)}, got {tuple(t.shape)}")
+    at = of_q[0].get_device()
+    for tensors, heads in ((of_q, n_heads), (of_kv, n_kv_heads)):
+        shape = (batch * seq_len, heads * head_dim)
+        for t in tensors:
+            if t.shape != shape or t.dtype != torch.bfloat16 or t.stride(1) != 1 or t.get_device() != at:
+                raise ValueError(f"a tensor of {heads} heads must be bf16 {shape} with unit inner stride on {of_q[0].device}, got {t.dtype} "
+                                 f"{tuple(t.shape)} on {t.device}")
     if not 0.0 <= softcap < math.inf:
         raise ValueError("softcap must be 0 or a finite cap")
     if spans is not None and (spans.batch, spans.seq) != (batch, seq_len):
         raise ValueError(f"spans are of {(spans.batch, spans.seq)}, not of {(batch, seq_len)}")
+    if spans is not None and spans.get_device() != at:
+        raise ValueError(f"spans are on {spans.device}")
     if slopes is not None:
-        _check_rows((("slopes", slopes, (n_heads,)),), torch.float32)
+        _check_like("slopes", torch.float32, (n_heads,), at, slopes)
     if lse is not None:
-        _check_rows((("lse", lse, (batch, n_heads, seq_len)),), torch.float32)
-    _check_here([(n, t) for n, t, _ in named] + [("spans", spans), ("slopes", slopes), ("lse", lse)])
+        _check_like("lse", torch.float32, (batch, n_heads, seq_len), at, lse)
+    _check_here(of_q[0])
 
 
 def attention_supported(seq_len: int, head_dim: int) -> bool:
@@ -1054,11 +1075,8 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: int,
     tanh(s / softcap)``; ``slopes`` (fp32 ``[n_heads]``, not differentiated) lower them by ``slope * |query - key|``.  With any of the
     three the sequence may have any length; a row that sees nothing gets zeros and a ``lse`` of -infinity.  Keys of another document
     that share a block of 128 with those of a row have to be finite; padding need not."""
-    for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
-        _check_2d_bf16(t, name)
     if spans is not None or softcap != 0.0 or slopes is not None:
-        _check_masked((("q", q, n_heads), ("k", k, n_kv_heads), ("v", v, n_kv_heads), ("out", out, n_heads)), spans, softcap, slopes, lse, batch,
-                      seq_len, n_heads, n_kv_heads, head_dim)
+        _check_masked((q, out), (k, v), spans, softcap, slopes, lse, batch, seq_len, n_heads, n_kv_heads, head_dim)
         if batch == 0 or seq_len == 0:
             return
         if not q.is_cuda:
@@ -1076,6 +1094,8 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: int,
             "attention_masked_fwd",
         )
         return
+    for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
+        _check_2d_bf16(t, name)
     if not q.is_cuda:
         B, S = batch, seq_len
         q4, k4, v4 = (t.reshape(B, S, -1, head_dim) for t in (q, k, v))
@@ -1143,12 +1163,12 @@ def attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Te
 
     ``spans``, ``softcap`` and ``slopes`` as in the forward pass; with any of them sequences have any length, the default
     ``scratch`` is this call's own, and rows that see nothing, or are seen by nobody, get zeros."""
-    for t, name in ((q, "q"), (k, "k"), (v, "v"), (o, "o"), (d_o, "d_o"), (dq, "dq"), (dk, "dk"), (dv, "dv")):
-        _check_2d_bf16(t, name)
     masked = spans is not None or softcap != 0.0 or slopes is not None
-    if masked:
-        _check_masked((("q", q, n_heads), ("k", k, n_kv_heads), ("v", v, n_kv_heads), ("o", o, n_heads), ("d_o", d_o, n_heads), ("dq", dq, n_heads),
-                       ("dk", dk, n_kv_heads), ("dv", dv, n_kv_heads)), spans, softcap, slopes, lse, batch, seq_len, n_heads, n_kv_heads, head_dim)
+    if not masked:
+        for t, name in ((q, "q"), (k, "k"), (v, "v"), (o, "o"), (d_o, "d_o"), (dq, "dq"), (dk, "dk"), (dv, "dv")):
+            _check_2d_bf16(t, name)
+    else:
+        _check_masked((q, o, d_o, dq), (k, v, dk, dv), spans, softcap, slopes, lse, batch, seq_len, n_heads, n_kv_heads, head_dim)
         if batch == 0 or seq_len == 0:
             return
         if not q.is_cuda:
