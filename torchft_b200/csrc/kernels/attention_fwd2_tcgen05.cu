@@ -33,17 +33,12 @@
 // Sequences of any length: the tensor maps have the sequence as a dimension of its own, so a tile's rows beyond its end are
 // zeros (not the next sequence's); keys there are masked, queries there are not stored.
 //
-// With MASK a query sees a range of keys of its own (attention_masks.cuh: documents, prefixes, windows), with SCORE its scores are capped by a
-// tanh or lowered by their distance first.  Both tiles of a CTA then walk over the same key blocks: they are two heads of a group at the same
-// queries where the group's size is even, and two query tiles of a head otherwise.
-//
 // Every mbarrier wait is bounded; on expiry the CTA records FTB200_ST_TIMEOUT in the caller's
 // status word, frees its TMEM and returns.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <math.h>
 
-#include "attention_masks.cuh"
 #include "ftb200_common.cuh"
 #include "tcgen05_helpers.cuh"
 
@@ -83,8 +78,6 @@ struct Attn2Params {
   float scale_log2;  // softmax scale * log2(e)
   float* lse;        // [batch, n_heads, seq], natural log
   int* status;
-  ftb200::MaskParams mask;  // of the kernels with MASK
-  int pair_heads;           // their two tiles are heads h and h + 1
 };
 
 enum : int {
@@ -100,7 +93,7 @@ enum : int {
   NUM_BARS = 18,
 };
 
-template <int D, int POLY, bool MASK, bool SCORE>
+template <int D, int POLY>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 attention_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const Attn2Params p) {
@@ -118,16 +111,17 @@ attention_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
   auto bar = [&](int i) { return bar_base + 8u * i; };
 
   // heavy (late) query blocks first: with a causal mask their work is largest
-  const bool pair_heads = MASK && p.pair_heads;
-  const int q_step = pair_heads ? 0 : BQ, h_step = pair_heads ? 1 : 0;  // from tile 0 to tile 1
-  const int cta_rows = pair_heads ? BQ : BQ * TILES, cta_heads = p.n_heads / (pair_heads ? TILES : 1);
-  const int n_qpairs = (p.seq + cta_rows - 1) / cta_rows;
-  const int per_block = p.batch * cta_heads;
+  const int n_qpairs = (p.seq + BQ * TILES - 1) / (BQ * TILES);
+  const int per_block = p.batch * p.n_heads;
   const int qp = n_qpairs - 1 - static_cast<int>(blockIdx.x) / per_block;
   const int bh = static_cast<int>(blockIdx.x) % per_block;
-  const int b = bh / cta_heads, h = bh % cta_heads * (pair_heads ? TILES : 1);
+  const int b = bh / p.n_heads, h = bh % p.n_heads;
   const int hk = h / (p.n_heads / p.n_kv_heads);
-  const int q0 = qp * cta_rows;  // first query in its sequence
+  // key blocks seen by tile 0 and tile 1
+  const int n_blocks = (p.seq + BKV - 1) / BKV;
+  const int n_kv0 = p.causal ? qp * TILES + 1 : n_blocks;
+  const int n_kv1 = p.causal ? min(qp * TILES + 2, n_blocks) : n_blocks;
+  const int q0 = qp * BQ * TILES;  // first query in its sequence
 
   if (threadIdx.x == 0) {
     for (int t = 0; t < TILES; ++t) {
@@ -160,27 +154,15 @@ attention_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
 
   ftb200::wait_for_previous();
 
-  // key blocks seen by tile 0 and tile 1, from block kb0 on
-  const int n_blocks = (p.seq + BKV - 1) / BKV;
-  int kb0 = 0, n_kv0, n_kv1;
-  if constexpr (MASK) {
-    const ftb200::KeyRange r = p.mask.keys_of(b, q0, pair_heads ? 1 : TILES, p.seq);
-    kb0 = r.lo / BKV;
-    n_kv0 = n_kv1 = r.hi > r.lo ? (r.hi + BKV - 1) / BKV - kb0 : 0;
-  } else {
-    n_kv0 = p.causal ? qp * TILES + 1 : n_blocks;
-    n_kv1 = p.causal ? min(qp * TILES + 2, n_blocks) : n_blocks;
-  }
-
   if (warp < 4) {
     regs_dec<ISSUE_REGS>();
     if (warp == 0) {
       // ---------------- TMA producer ----------------
-      if (elect_one() && n_kv1 > 0) for (int t = 0; t < TILES; ++t) {
+      if (elect_one()) for (int t = 0; t < TILES; ++t) {
         const uint32_t sq = smem_base + C::OFF_Q + t * C::TILE_BYTES;
         mbar_expect_tx(bar(BAR_Q_FULL + t), C::TILE_BYTES);
         for (int s = 0; s < C::SLABS; ++s)
-          tma_load_3d(sq + s * C::SLAB_BYTES, &tmQ, bar(BAR_Q_FULL + t), (h + t * h_step) * D + s * 64, q0 + t * q_step, b);
+          tma_load_3d(sq + s * C::SLAB_BYTES, &tmQ, bar(BAR_Q_FULL + t), h * D + s * 64, q0 + t * BQ, b);
       }
       bool ok = true;
       for (int j = 0; j < n_kv1 && ok; ++j) {
@@ -192,7 +174,7 @@ attention_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         }
         const uint32_t sk = smem_base + C::OFF_KV + st * 2 * C::TILE_BYTES;
         const uint32_t sv = sk + C::TILE_BYTES;
-        const int kv0 = (kb0 + j) * BKV;
+        const int kv0 = j * BKV;
         if (elect_one()) {
           mbar_expect_tx(bar(BAR_K_FULL + st), C::TILE_BYTES);
           for (int s = 0; s < C::SLABS; ++s) tma_load_3d(sk + s * C::SLAB_BYTES, &tmK, bar(BAR_K_FULL + st), hk * D + s * 64, kv0, b);
@@ -257,21 +239,13 @@ attention_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         }
         __syncwarp();
       };
-      const bool padded = MASK && p.mask.has_padding(b, p.seq, lane);
-      bool ok = n_kv1 > 0 && mbar_wait_warp(bar(BAR_Q_FULL + 0), 0, abort_flag) && mbar_wait_warp(bar(BAR_K_FULL + 0), 0, abort_flag);
-      // what stands in padding reaches neither the products nor the choice of a way for the scores
-      auto clear = [&](uint32_t off, int tile) {
-        if (padded && tile < n_blocks) p.mask.clear_padding(smem + off, C::SLABS, b, tile, p.seq, lane);
-      };
+      bool ok = mbar_wait_warp(bar(BAR_Q_FULL + 0), 0, abort_flag) && mbar_wait_warp(bar(BAR_K_FULL + 0), 0, abort_flag);
       if (ok) {
-        clear(C::OFF_Q, q0 / BQ);
-        clear(C::OFF_KV, kb0);
         tc_fence_after();
         issue_s(0, 0);
         ok = mbar_wait_warp(bar(BAR_Q_FULL + 1), 0, abort_flag);
       }
       if (ok) {
-        clear(C::OFF_Q + C::TILE_BYTES, (q0 + q_step) / BQ);
         tc_fence_after();
         issue_s(1, 0);
         if (elect_one()) umma_commit(bar(BAR_K_EMPTY + 0));
@@ -286,7 +260,6 @@ attention_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
             ok = false;
             break;
           }
-          clear(C::OFF_KV + st * 2 * C::TILE_BYTES + C::TILE_BYTES, kb0 + j);
           tc_fence_after();
           issue_pv(0, j, 0);
           if (!mbar_wait_warp(bar(BAR_P_FULL + 0), static_cast<uint32_t>(j) & 1u, abort_flag)) {
@@ -302,7 +275,6 @@ attention_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
               break;
             }
             k_next = true;
-            clear(C::OFF_KV + st1 * 2 * C::TILE_BYTES, kb0 + j + 1);
             tc_fence_after();
             issue_s(0, j + 1);
           }
@@ -343,14 +315,6 @@ attention_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     const uint32_t s_addr = tmem_base + C::COL_S + t * 128 + lane_addr;
     const uint32_t o_addr = tmem_base + C::COL_O + t * D + lane_addr;
     const int n_kv = t == 0 ? n_kv0 : n_kv1;
-    const int query = q0 + t * q_step + row;
-    const int head = h + t * h_step;
-    ftb200::RowMask mine = {0, 0, 0, 0};
-    float slope2 = 0.f;
-    if constexpr (MASK) mine = p.mask.row(b, query, p.seq);
-    if constexpr (SCORE) slope2 = p.mask.slope2(head);
-    // with SCORE the scores come scaled, in units of log2
-    const float scale_log2 = SCORE ? 1.f : p.scale_log2;
     float m_used = -INFINITY, l_sum = 0.f;
     bool ok = true;
     for (int j = 0; j < n_kv; ++j) {
@@ -363,22 +327,7 @@ attention_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
 #pragma unroll
       for (int c = 0; c < BKV / 32; ++c) tmem_ld32(s_addr + c * 32, sv + c * 32);
       tmem_wait_ld();
-      if constexpr (SCORE) {
-        p.mask.cap_scores<BKV>(sv);
-        p.mask.slope_scores<BKV>(sv, static_cast<float>(query - (kb0 + j) * BKV), -1.f, slope2);
-      }
-      if constexpr (MASK) {
-        const int first = (kb0 + j) * BKV;
-        if (!mine.all(first, BKV)) {
-#pragma unroll
-          for (int w = 0; w < BKV / 32; ++w) {
-            const uint32_t bits = ftb200::range_bits(mine.lo - first - 32 * w, mine.hi - first - 32 * w);
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (!(bits >> c & 1u)) sv[32 * w + c] = __float_as_uint(-INFINITY);
-          }
-        }
-      } else if (p.causal && j == n_kv - 1) {
+      if (p.causal && j == n_kv - 1) {
         // the diagonal block: key c of the block is visible to query `row` of the tile iff c <= row
 #pragma unroll
         for (int c = 0; c < BKV; ++c)
@@ -397,12 +346,12 @@ attention_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
 
       // raise the maximum only when it moved far
       float alpha = 1.f;
-      const bool raise = j > 0 && (m_new - m_used) * scale_log2 > RESCALE_THRESHOLD;
+      const bool raise = j > 0 && (m_new - m_used) * p.scale_log2 > RESCALE_THRESHOLD;
       const bool any_raise = __any_sync(0xffffffffu, raise);
       if (j == 0) {
         m_used = m_new;
       } else if (raise) {
-        alpha = exp2f((m_used - m_new) * scale_log2);
+        alpha = exp2f((m_used - m_new) * p.scale_log2);
         m_used = m_new;
         l_sum *= alpha;
       }
@@ -423,9 +372,8 @@ attention_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
           tmem_st32(o_addr + c * 32, ov);
         }
       }
-      // a row that has seen nothing yet has no maximum
-      const float neg_m = MASK && m_used == -INFINITY ? 0.f : -m_used * scale_log2;
-      const unsigned long long scale2 = f2_pack(scale_log2, scale_log2), neg_m2 = f2_pack(neg_m, neg_m);
+      const float neg_m = -m_used * p.scale_log2;
+      const unsigned long long scale2 = f2_pack(p.scale_log2, p.scale_log2), neg_m2 = f2_pack(neg_m, neg_m);
       unsigned long long sum2[2] = {0ull, 0ull};
 #pragma unroll
       for (int c = 0; c < BKV / 32; ++c) {
@@ -466,12 +414,12 @@ attention_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
       mbar_arrive_warp(bar(BAR_P_FULL + t));
     }
 
-    if (ok && ((MASK && n_kv == 0) || mbar_wait_warp(bar(BAR_O_DONE + t), static_cast<uint32_t>(n_kv - 1) & 1u, abort_flag))) {
+    if (ok && mbar_wait_warp(bar(BAR_O_DONE + t), static_cast<uint32_t>(n_kv - 1) & 1u, abort_flag)) {
       tc_fence_after();
-      const bool nothing = MASK && l_sum == 0.f;  // no key is seen: zeros, and a log-sum-exp of -infinity
       const float inv = 1.f / l_sum;
+      const int query = q0 + t * BQ + row;
       // O leaves by TMA, 32 rows a warp, from the place of this tile's Q, whose last product is done.  Stored by the threads, 16 bytes of 32 rows an
-      // instruction, it held every CTA up for 9.2 us.
+      // instruction, it held every CTA up for 9.2 us (1.2 now).
       uint8_t* stage = smem + C::OFF_Q + t * C::TILE_BYTES + row * 128;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
@@ -482,23 +430,23 @@ attention_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         for (int q4 = 0; q4 < 4; ++q4) {
           float f[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] = nothing ? 0.f : __uint_as_float(ov[8 * q4 + e]) * inv;
+          for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(ov[8 * q4 + e]) * inv;
           *reinterpret_cast<ftb200::bf16x8*>(stage + (c >> 1) * C::SLAB_BYTES + ((((c & 1) * 4 + q4) ^ (row & 7)) << 4)) = ftb200::pack8(f);
         }
       }
       fence_async_smem();
       __syncwarp();
-      const int first = q0 + t * q_step + quarter * 32;
+      const int first = q0 + t * BQ + quarter * 32;
       if (first < p.seq && elect_one()) {
         for (int s = 0; s < C::SLABS; ++s)
-          tma_store_3d(&tmO, smem_base + C::OFF_Q + t * C::TILE_BYTES + s * C::SLAB_BYTES + quarter * (32 * 128), head * D + s * 64, first, b);
+          tma_store_3d(&tmO, smem_base + C::OFF_Q + t * C::TILE_BYTES + s * C::SLAB_BYTES + quarter * (32 * 128), h * D + s * 64, first, b);
         bulk_commit();
         bulk_wait_read();
       }
       __syncwarp();
       if (p.lse != nullptr && query < p.seq) {
-        p.lse[(static_cast<long long>(b) * p.n_heads + head) * p.seq + query] =
-            nothing ? -INFINITY : (m_used * scale_log2 + log2f(l_sum)) * 0.6931471805599453f;
+        p.lse[(static_cast<long long>(b) * p.n_heads + h) * p.seq + query] =
+            (m_used * p.scale_log2 + log2f(l_sum)) * 0.6931471805599453f;
       }
     }
   }
@@ -541,41 +489,24 @@ int encode_rows2(CUtensorMap* map, const void* base, long long batch, long long 
   return r == CUDA_SUCCESS ? 0 : FTB200_E_DRIVER;
 }
 
-struct Maps {
-  CUtensorMap q, k, v, o;
-};
-
-template <int D, int POLY, bool MASK = false, bool SCORE = false>
-int launch_fwd2(const Maps& m, const Attn2Params& p, long long grid, cudaStream_t stream) {
-  auto* kernel = attention_fwd2_kernel<D, POLY, MASK, SCORE>;
+template <int D, int POLY>
+int launch_fwd2(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to, const Attn2Params& p, long long grid,
+                cudaStream_t stream) {
   static bool attr_set = false;
   if (!attr_set) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM_BYTES) != cudaSuccess)
+    if (cudaFuncSetAttribute(attention_fwd2_kernel<D, POLY>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             Cfg<D>::SMEM_BYTES) != cudaSuccess)
       return FTB200_E_CUDA;
     // The warpgroups' register split assumes this count, which the compiler gives a kernel that moves registers; with fewer
     // the softmax warpgroups would wait for registers that nobody has.
     cudaFuncAttributes attr;
-    if (cudaFuncGetAttributes(&attr, kernel) != cudaSuccess) return FTB200_E_CUDA;
+    if (cudaFuncGetAttributes(&attr, attention_fwd2_kernel<D, POLY>) != cudaSuccess) return FTB200_E_CUDA;
     if (attr.numRegs < LAUNCH_REGS) return FTB200_E_REGS;
     attr_set = true;
   }
-  ftb200::launch_after(kernel, static_cast<unsigned>(grid), NUM_THREADS, Cfg<D>::SMEM_BYTES, stream, m.q, m.k, m.v, m.o, p);
+  ftb200::launch_after(attention_fwd2_kernel<D, POLY>, static_cast<unsigned>(grid), NUM_THREADS, Cfg<D>::SMEM_BYTES, stream,
+      tq, tk, tv, to, p);
   return cudaGetLastError() == cudaSuccess ? 0 : FTB200_E_CUDA;
-}
-
-int make_maps(Maps* m, const void* q, const void* k, const void* v, const void* o, int batch, int seq, int n_heads, int n_kv_heads, int head_dim,
-              long long ld_q, long long ld_k, long long ld_v, long long ld_o) {
-  if ((head_dim != 64 && head_dim != 128) || batch <= 0 || seq <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0)
-    return FTB200_E_BADARG;
-  auto aligned16 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
-  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || (ld_q & 7) || (ld_k & 7) || (ld_v & 7) ||
-      (ld_o & 7))
-    return FTB200_E_ALIGN;
-  int rc = encode_rows2(&m->q, q, batch, seq, static_cast<long long>(n_heads) * head_dim, ld_q);
-  if (rc == 0) rc = encode_rows2(&m->k, k, batch, seq, static_cast<long long>(n_kv_heads) * head_dim, ld_k);
-  if (rc == 0) rc = encode_rows2(&m->v, v, batch, seq, static_cast<long long>(n_kv_heads) * head_dim, ld_v);
-  if (rc == 0) rc = encode_rows2(&m->o, o, batch, seq, static_cast<long long>(n_heads) * head_dim, ld_o, 32);
-  return rc;
 }
 
 }  // namespace
@@ -588,48 +519,31 @@ FTB200_API int ftb200_attention_fwd2(const void* q, const void* k, const void* v
                                      int n_heads, int n_kv_heads, int head_dim, long long ld_q, long long ld_k,
                                      long long ld_v, long long ld_o, float scale, int causal, int poly, int* status,
                                      cudaStream_t stream) {
-  if (poly != 0 && poly != 2 && poly != 4) return FTB200_E_BADARG;
-  Maps m;
-  const int rc = make_maps(&m, q, k, v, o, batch, seq, n_heads, n_kv_heads, head_dim, ld_q, ld_k, ld_v, ld_o);
+  if ((head_dim != 64 && head_dim != 128) || batch <= 0 || seq <= 0 || n_heads <= 0 ||
+      n_kv_heads <= 0 || n_heads % n_kv_heads != 0 || (poly != 0 && poly != 2 && poly != 4))
+    return FTB200_E_BADARG;
+  auto aligned16 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || (ld_q & 7) || (ld_k & 7) || (ld_v & 7) ||
+      (ld_o & 7))
+    return FTB200_E_ALIGN;
+  CUtensorMap tq, tk, tv, to;
+  int rc = encode_rows2(&tq, q, batch, seq, static_cast<long long>(n_heads) * head_dim, ld_q);
+  if (rc == 0) rc = encode_rows2(&tk, k, batch, seq, static_cast<long long>(n_kv_heads) * head_dim, ld_k);
+  if (rc == 0) rc = encode_rows2(&tv, v, batch, seq, static_cast<long long>(n_kv_heads) * head_dim, ld_v);
+  if (rc == 0) rc = encode_rows2(&to, o, batch, seq, static_cast<long long>(n_heads) * head_dim, ld_o, 32);
   if (rc != 0) return rc;
-  Attn2Params p = {};
+  Attn2Params p;
   p.batch = batch; p.seq = seq; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads; p.causal = causal;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.lse = lse; p.status = status;
   const long long grid = static_cast<long long>(batch) * n_heads * ((static_cast<long long>(seq) + BQ * TILES - 1) / (BQ * TILES));
   if (grid > 0x7fffffffLL) return FTB200_E_TOOBIG;
   if (head_dim == 128) {
-    if (poly == 0) return launch_fwd2<128, 0>(m, p, grid, stream);
-    if (poly == 2) return launch_fwd2<128, 2>(m, p, grid, stream);
-    return launch_fwd2<128, 4>(m, p, grid, stream);
+    if (poly == 0) return launch_fwd2<128, 0>(tq, tk, tv, to, p, grid, stream);
+    if (poly == 2) return launch_fwd2<128, 2>(tq, tk, tv, to, p, grid, stream);
+    return launch_fwd2<128, 4>(tq, tk, tv, to, p, grid, stream);
   }
-  if (poly == 0) return launch_fwd2<64, 0>(m, p, grid, stream);
-  if (poly == 2) return launch_fwd2<64, 2>(m, p, grid, stream);
-  return launch_fwd2<64, 4>(m, p, grid, stream);
-}
-
-// The same under a mask (attention_masks.cuh).  rows, tiles, padded: null, where every query sees the keys up to its own (causal) or all, or what
-// ftb200_attention_spans wrote.  softcap: 0, or what the scores are capped at, softcap tanh(scale s / softcap).  slopes: null, or [n_heads]
-// fp32: slope |query - key| is subtracted from a score.
-FTB200_API int ftb200_attention_masked_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const void* rows, const void* tiles,
-                                           const int* padded, const float* slopes, int batch, int seq, int n_heads, int n_kv_heads, int head_dim,
-                                           long long ld_q, long long ld_k, long long ld_v, long long ld_o, float scale, float softcap, int causal,
-                                           int* status, cudaStream_t stream) {
-  Maps m;
-  int rc = make_maps(&m, q, k, v, o, batch, seq, n_heads, n_kv_heads, head_dim, ld_q, ld_k, ld_v, ld_o);
-  Attn2Params p = {};
-  if (rc == 0) rc = ftb200::set_mask(&p.mask, rows, tiles, padded, slopes, scale, softcap, causal, seq);
-  if (rc != 0) return rc;
-  p.batch = batch; p.seq = seq; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads; p.causal = causal;
-  p.scale_log2 = scale * 1.4426950408889634f;
-  p.lse = lse; p.status = status;
-  p.pair_heads = n_heads / n_kv_heads % TILES == 0;
-  const long long tiles_q = (static_cast<long long>(seq) + BQ - 1) / BQ;
-  const long long grid = p.pair_heads ? batch * (static_cast<long long>(n_heads) / TILES) * tiles_q
-                                      : static_cast<long long>(batch) * n_heads * ((tiles_q + TILES - 1) / TILES);
-  if (grid > 0x7fffffffLL) return FTB200_E_TOOBIG;
-  const bool score = softcap > 0.f || slopes != nullptr;
-  if (head_dim == 128)
-    return score ? launch_fwd2<128, 0, true, true>(m, p, grid, stream) : launch_fwd2<128, 0, true, false>(m, p, grid, stream);
-  return score ? launch_fwd2<64, 0, true, true>(m, p, grid, stream) : launch_fwd2<64, 2, true, false>(m, p, grid, stream);
+  if (poly == 0) return launch_fwd2<64, 0>(tq, tk, tv, to, p, grid, stream);
+  if (poly == 2) return launch_fwd2<64, 2>(tq, tk, tv, to, p, grid, stream);
+  return launch_fwd2<64, 4>(tq, tk, tv, to, p, grid, stream);
 }

@@ -1,0 +1,655 @@
+// Grouped-query attention, forward pass, under a mask of ranges and with changed scores (attention_masks.cuh).
+//
+//   O[b, s, h, :] = softmax(y(Q[b, s, h, :] K[b, :, h / group, :]^T), over the keys that query s sees) V[b, :, h / group, :]
+//
+// head_dim 64 or 128, bf16 in/out, fp32 accumulation and statistics.  Q, K and V are read in place from a packed
+// [batch * seq, n_cols] activation (any row stride).
+//
+// An item of work is one (batch, pair of tiles of 128 queries): two heads of a group at the same queries where the group's size is even, so that
+// the tiles look at the same keys, and two query tiles of a head otherwise.  Both walk over the 64-key blocks that some query of them sees.
+// Documents make items short (8 blocks of 128 keys where 1000 tokens are a document) and unequal, so what surrounds them counts as much as
+// their loop:
+//
+//   - a CTA per SM stays and takes items one after another, in the grid's order, by cancelling CTAs that have not been launched yet (cluster
+//     launch control), the next one when its current item is nearly done; the next item's Q, K and first products are under way while the
+//     current one's output leaves.  As a CTA of its own an item of one key block took 8.6 us, of which 1.4 in the softmax;
+//   - the scores of a tile have two buffers of 64 keys each, so that a block's product S = Q K^T runs while the softmax works on the one
+//     before: with one buffer of 128 keys the softmax waited 1224 of 3552 cycles for P V and the next S;
+//   - blocks that each query sees need no mask; in the others a row's seen keys are a run of bits.
+//
+//   warp 0        TMA: Q tiles of an item, K and V blocks of 128 keys into a 2-stage ring
+//   warps 1, 3    tcgen05.mma of a tile each, per block of 64 keys: P V, then S of the block after the next.  (One warp for both spent
+//                 220 cycles and more on every wait, beside two softmax warps, and was what bounded the loop.)
+//   warp 2        the next item: launch control, the range of its keys
+//   warps 4..7    softmax and output of tile 0, warps 8..11 of tile 1: one thread per query row
+//
+// The running maximum is only raised (and O in TMEM rescaled) when it grows by more than 2^8.  P goes back as packed bf16 into the first 32
+// columns of the scores it came from and is the A operand of P V straight from tensor memory.
+//
+// Sequences of any length: the tensor maps have the sequence as a dimension of its own, so a tile's rows beyond its end are zeros (not the
+// next sequence's); keys there are in no query's range, queries there are not stored.
+//
+// Every mbarrier wait is bounded; on expiry the CTA records FTB200_ST_TIMEOUT in the caller's status word, frees its TMEM and returns.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <math.h>
+
+#include "attention_masks.cuh"
+#include "ftb200_common.cuh"
+#include "tcgen05_helpers.cuh"
+
+namespace {
+
+using namespace ftb200::tc;
+
+constexpr int BQ = 128;    // queries per tile
+constexpr int TILES = 2;   // tiles per item
+constexpr int BKV = 128;   // keys per stage of K and V
+constexpr int SUB = 64;    // keys per step of the softmax
+constexpr int STAGES = 2;  // of K and V, of the scores, and of the items
+constexpr int NUM_THREADS = 384;
+// Registers: a CTA is launched with 168 a thread (65536 / 384, checked on the host); the first warpgroup gives most of its own to the two
+// softmax warpgroups: 72 + 2 * 216 = 3 * 168.
+constexpr int LAUNCH_REGS = 168, ISSUE_REGS = 72, SOFTMAX_REGS = 216;
+static_assert(ISSUE_REGS + 2 * SOFTMAX_REGS <= 3 * LAUNCH_REGS, "more registers than the CTA is launched with");
+constexpr int ROW_WARPS = 4;                  // softmax warps per tile
+constexpr int READERS = 1 + TILES + TILES * ROW_WARPS;  // warps that read an item
+constexpr int CLAIM_AHEAD = 6;                // steps before its end at which an item asks for the next one
+constexpr uint32_t TMEM_COLS = 512;
+constexpr float RESCALE_THRESHOLD = 8.0f;  // in log2 units
+
+template <int D>
+struct Cfg {
+  static constexpr uint32_t TILE_BYTES = 128 * D * 2;  // a 128-row operand tile
+  static constexpr uint32_t SLAB_BYTES = 128 * 128;    // 128 rows x 64 elements (one swizzle atom wide)
+  static constexpr int SLABS = D / 64;
+  static constexpr uint32_t OFF_Q = 0;                    // Q0 Q1
+  static constexpr uint32_t OFF_KV = TILES * TILE_BYTES;  // K0 V0 | K1 V1
+  static constexpr uint32_t OFF_O = OFF_KV + STAGES * 2 * TILE_BYTES;  // per softmax warp: 32 rows x 64 elements on their way out
+  static constexpr uint32_t OFF_MISC = OFF_O + TILES * ROW_WARPS * 4096;
+  static constexpr uint32_t SMEM_BYTES = OFF_MISC + 512 + 1024;
+  static_assert(SMEM_BYTES <= 232448, "exceeds the 227 KB of shared memory a CTA can have");
+  static constexpr uint32_t COL_S = 0;    // S of tile t, buffer s at COL_S + t * 128 + s * 64
+  static constexpr uint32_t COL_O = 256;  // O_t at COL_O + t * D
+};
+
+struct Params {
+  int batch, seq, n_heads, n_kv_heads;
+  int pair_heads;  // an item's tiles are heads h and h + 1
+  float scale_log2;  // softmax scale * log2(e)
+  float* lse;        // null, or [batch, n_heads, seq], natural log
+  int* status;
+  ftb200::MaskParams mask;
+};
+
+struct Item {
+  int batch;  // below zero: there is none
+  int head, query;
+  int first, steps;  // blocks of 64 keys
+};
+
+enum : int {
+  BAR_Q_FULL = 0,     // +tile
+  BAR_Q_EMPTY = 2,    // +tile
+  BAR_K_FULL = 4,     // +stage
+  BAR_K_EMPTY = 6,    // +stage
+  BAR_V_FULL = 8,     // +stage
+  BAR_V_EMPTY = 10,   // +stage
+  BAR_S_FULL = 12,    // +2 tile + buffer
+  BAR_P_FULL = 16,    // +2 tile + buffer
+  BAR_O_DONE = 20,    // +tile: P V of a step
+  BAR_O_FREE = 22,    // +tile: O has been read
+  BAR_ITEM_FULL = 24,   // +slot
+  BAR_ITEM_EMPTY = 26,  // +slot
+  BAR_CLAIM = 28,     // the current item is nearly done
+  BAR_CLAIMED = 29,   // the answer of the launch control
+  BAR_O_LAST = 30,    // +tile: P V of an item's last step (who waits for it may be two steps behind, which a parity does not tell apart)
+  NUM_BARS = 32,
+};
+
+// The grid's next CTA that has not been launched, or -1: the answer (16 bytes) arrives in shared memory with the barrier.
+__device__ __forceinline__ void claim_next(uint32_t answer, uint32_t bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar) : "memory");
+}
+__device__ __forceinline__ int claimed(uint32_t answer) {
+  uint32_t ok, x;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      ".reg .b128 c;\n"
+      "ld.shared.b128 c, [%2];\n"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, c;\n"
+      "selp.u32 %0, 1, 0, p;\n"
+      "mov.u32 %1, 0;\n"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, c;\n"
+      "}\n"
+      : "=r"(ok), "=r"(x)
+      : "r"(answer)
+      : "memory");
+  return ok ? static_cast<int>(x) : -1;
+}
+
+template <int D, int POLY, bool SCORE>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+attention_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                            const __grid_constant__ CUtensorMap tmO, const Params p) {
+  using C = Cfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_MISC);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC + 256);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 260);
+  Item* items = reinterpret_cast<Item*>(smem + C::OFF_MISC + 288);  // two slots
+  static_assert(NUM_BARS * 8 <= 256 && 288 + 2 * sizeof(Item) <= 384, "barriers, slots and the answer overlap");
+
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
+  const uint32_t smem_base = smem_u32(smem);
+  const uint32_t bar_base = smem_u32(bars);
+  const uint32_t answer = smem_base + C::OFF_MISC + 384;
+  auto bar = [&](int i) { return bar_base + 8u * i; };
+  auto wait = [&](int which, uint32_t parity) { return mbar_wait_warp(bar(which), parity & 1u, abort_flag); };
+
+  const int rep = p.n_heads / p.n_kv_heads;
+  const int q_step = p.pair_heads ? 0 : BQ, h_step = p.pair_heads ? 1 : 0;  // from tile 0 to tile 1
+
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < TILES; ++t) {
+      mbar_init(bar(BAR_Q_FULL + t), 1);
+      mbar_init(bar(BAR_Q_EMPTY + t), 1);
+      mbar_init(bar(BAR_O_DONE + t), 1);
+      mbar_init(bar(BAR_O_LAST + t), 1);
+      mbar_init(bar(BAR_O_FREE + t), ROW_WARPS);
+      for (int s = 0; s < STAGES; ++s) {
+        mbar_init(bar(BAR_S_FULL + 2 * t + s), 1);
+        mbar_init(bar(BAR_P_FULL + 2 * t + s), ROW_WARPS);
+      }
+    }
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(bar(BAR_K_FULL + s), 1);
+      mbar_init(bar(BAR_K_EMPTY + s), TILES);
+      mbar_init(bar(BAR_V_FULL + s), 1);
+      mbar_init(bar(BAR_V_EMPTY + s), TILES);
+      mbar_init(bar(BAR_ITEM_FULL + s), 1);
+      mbar_init(bar(BAR_ITEM_EMPTY + s), READERS);
+    }
+    mbar_init(bar(BAR_CLAIM), 1);
+    mbar_init(bar(BAR_CLAIMED), 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+
+  ftb200::wait_for_previous();
+
+  // Item number k of this CTA, for one of the READERS: false where the CTA is aborting.
+  auto read_item = [&](int k, Item& it) {
+    if (!wait(BAR_ITEM_FULL + (k & 1), k >> 1)) return false;
+    const Item& at = items[k & 1];
+    // from lane 0, so that what depends on it, the MMAs' descriptors above all, is known to be the same in all lanes and stays in uniform registers
+    auto same = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+    it = {same(at.batch), same(at.head), same(at.query), same(at.first), same(at.steps)};
+    mbar_arrive_warp(bar(BAR_ITEM_EMPTY + (k & 1)));
+    return true;
+  };
+  // the stage of K and V that step i lies in, counted from the item's first
+  auto stage_of = [](const Item& it, int i) { return ((it.first + i) >> 1) - (it.first >> 1); };
+
+  if (warp < 4) {
+    regs_dec<ISSUE_REGS>();
+    if (warp == 0) {
+      // ---------------- TMA producer ----------------
+      bool ok = true;
+      int blocks = 0, full = 0;  // stages and items with keys, so far
+      for (int k = 0; ok; ++k) {
+        Item it;
+        if (!(ok = read_item(k, it)) || it.batch < 0) break;
+        if (it.steps == 0) continue;
+        const int hk = it.head / rep;
+        for (int t = 0; t < TILES && ok; ++t) {
+          if (!(ok = wait(BAR_Q_EMPTY + t, full ^ 1))) break;
+          if (elect_one()) {
+            const uint32_t sq = smem_base + C::OFF_Q + t * C::TILE_BYTES;
+            mbar_expect_tx(bar(BAR_Q_FULL + t), C::TILE_BYTES);
+            for (int s = 0; s < C::SLABS; ++s)
+              tma_load_3d(sq + s * C::SLAB_BYTES, &tmQ, bar(BAR_Q_FULL + t), (it.head + t * h_step) * D + s * 64, it.query + t * q_step, it.batch);
+          }
+          __syncwarp();
+          if (t > 0) break;
+          // the first block of keys between the two
+          const int st = blocks & 1;
+          if (!(ok = wait(BAR_K_EMPTY + st, (blocks >> 1) ^ 1))) break;
+          if (elect_one()) {
+            const uint32_t sk = smem_base + C::OFF_KV + st * 2 * C::TILE_BYTES;
+            mbar_expect_tx(bar(BAR_K_FULL + st), C::TILE_BYTES);
+            for (int s = 0; s < C::SLABS; ++s)
+              tma_load_3d(sk + s * C::SLAB_BYTES, &tmK, bar(BAR_K_FULL + st), hk * D + s * 64, (it.first >> 1) * BKV, it.batch);
+          }
+          __syncwarp();
+        }
+        const int n = stage_of(it, it.steps - 1) + 1;
+        for (int j = 0; j < n && ok; ++j, ++blocks) {
+          const int st = blocks & 1, use = blocks >> 1;
+          const uint32_t sk = smem_base + C::OFF_KV + st * 2 * C::TILE_BYTES;
+          const int key = ((it.first >> 1) + j) * BKV;
+          if (j > 0) {
+            if (!(ok = wait(BAR_K_EMPTY + st, use ^ 1))) break;
+            if (elect_one()) {
+              mbar_expect_tx(bar(BAR_K_FULL + st), C::TILE_BYTES);
+              for (int s = 0; s < C::SLABS; ++s) tma_load_3d(sk + s * C::SLAB_BYTES, &tmK, bar(BAR_K_FULL + st), hk * D + s * 64, key, it.batch);
+            }
+            __syncwarp();
+          }
+          if (!(ok = wait(BAR_V_EMPTY + st, use ^ 1))) break;
+          if (elect_one()) {
+            mbar_expect_tx(bar(BAR_V_FULL + st), C::TILE_BYTES);
+            for (int s = 0; s < C::SLABS; ++s)
+              tma_load_3d(sk + C::TILE_BYTES + s * C::SLAB_BYTES, &tmV, bar(BAR_V_FULL + st), hk * D + s * 64, key, it.batch);
+          }
+          __syncwarp();
+        }
+        ++full;
+      }
+      ftb200::start_next();
+      if (!ok) {
+        // copies in flight land in this CTA's shared memory: give them time before the CTA exits
+        const uint64_t t0 = ftb200::globaltimer_ns();
+        while (ftb200::globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+      }
+    } else if (warp != 2) {
+      // ---------------- MMA issuers: warp 1 for tile 0, warp 3 for tile 1 ----------------
+      const int t = warp >> 1;
+      // S = Q K^T: both operands K-major (head dim contiguous), M = 128, N = 64
+      const uint32_t F = (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(BQ >> 4) << 24);
+      const uint32_t idesc_s = F | (static_cast<uint32_t>(SUB >> 3) << 17);
+      // O += P V: A = P from tensor memory (keys contiguous), B = V MN-major (stored [key][d]), N = D
+      const uint32_t idesc_o = F | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17);
+      constexpr uint32_t HI = smem_desc_hi(1024);
+      constexpr uint32_t HALF16 = (SUB * 128) >> 4;  // the second 64 keys of a stage
+      const uint32_t q_lo = smem_desc_lo(smem_base + C::OFF_Q + t * C::TILE_BYTES, 16);
+      const uint32_t k_lo = smem_desc_lo(smem_base + C::OFF_KV, 16);
+      const uint32_t v_lo = smem_desc_lo(smem_base + C::OFF_KV + C::TILE_BYTES, C::SLAB_BYTES);
+      constexpr uint32_t STAGE16 = (2 * C::TILE_BYTES) >> 4;
+      bool ok = true;
+      int steps = 0, blocks = 0, full = 0;
+      for (int k = 0; ok; ++k) {
+        Item it;
+        if (!(ok = read_item(k, it)) || it.batch < 0) break;
+        if (it.steps == 0) {
+          if (t == 0 && elect_one()) mbar_arrive(bar(BAR_CLAIM));
+          __syncwarp();
+          continue;
+        }
+        const bool padded = p.mask.has_padding(it.batch, p.seq, lane);
+        // what stands in padding reaches neither the products nor the choice of a way for the scores
+        auto clear = [&](uint32_t off, int row) {
+          if (padded && row < p.seq) p.mask.clear_padding(smem + off, C::SLABS, it.batch, row / 128, p.seq, lane);
+        };
+        auto opens = [&](int i) { return i == 0 || ((it.first + i) & 1) == 0; };
+        auto closes = [&](int i) { return i == it.steps - 1 || ((it.first + i) & 1) != 0; };
+        auto issue_s = [&](int i) {
+          const int g = steps + i, blk = blocks + stage_of(it, i), st = blk & 1;
+          if (opens(i)) {
+            if (!wait(BAR_K_FULL + st, blk >> 1)) return false;
+            clear(C::OFF_KV + st * 2 * C::TILE_BYTES, ((it.first + i) >> 1) * BKV);
+          }
+          tc_fence_after();
+          const uint32_t kb = k_lo + st * STAGE16 + ((it.first + i) & 1) * HALF16;
+          const uint32_t d_tmem = tmem_base + C::COL_S + t * 128 + (g & 1) * SUB;
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t off = ((kk >> 2) * C::SLAB_BYTES + (kk & 3) * 32) >> 4;
+              umma_bf16_lh(d_tmem, q_lo + off, HI, kb + off, HI, idesc_s, kk != 0);
+            }
+            umma_commit(bar(BAR_S_FULL + 2 * t + (g & 1)));
+            if (i == it.steps - 1) umma_commit(bar(BAR_Q_EMPTY + t));
+            if (closes(i)) umma_commit(bar(BAR_K_EMPTY + st));
+          }
+          __syncwarp();
+          return true;
+        };
+        if (!(ok = wait(BAR_Q_FULL + t, full))) break;
+        clear(C::OFF_Q + t * C::TILE_BYTES, it.query + t * q_step);
+        ok = issue_s(0) && (it.steps == 1 || issue_s(1));
+        for (int i = 0; i < it.steps && ok; ++i) {
+          if (t == 0 && i == max(0, it.steps - CLAIM_AHEAD)) {
+            if (elect_one()) mbar_arrive(bar(BAR_CLAIM));
+            __syncwarp();
+          }
+          const int g = steps + i, blk = blocks + stage_of(it, i), st = blk & 1;
+          if (opens(i)) {
+            if (!(ok = wait(BAR_V_FULL + st, blk >> 1))) break;
+            clear(C::OFF_KV + st * 2 * C::TILE_BYTES + C::TILE_BYTES, ((it.first + i) >> 1) * BKV);
+          }
+          if (i == 0 && full > 0 && !(ok = wait(BAR_O_FREE + t, full - 1))) break;
+          if (!(ok = wait(BAR_P_FULL + 2 * t + (g & 1), g >> 1))) break;
+          tc_fence_after();
+          const uint32_t vb = v_lo + st * STAGE16 + ((it.first + i) & 1) * HALF16;
+          const uint32_t d_tmem = tmem_base + C::COL_O + t * D;
+          const uint32_t p_tmem = tmem_base + C::COL_S + t * 128 + (g & 1) * SUB;  // P: keys 2k, 2k+1 in column k
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < SUB / 16; ++kk) umma_bf16_tmem_a(d_tmem, p_tmem + kk * 8, vb + ((kk * 2048) >> 4), HI, idesc_o, (i | kk) != 0);
+            umma_commit(bar(BAR_O_DONE + t));
+            if (i == it.steps - 1) umma_commit(bar(BAR_O_LAST + t));
+            if (closes(i)) umma_commit(bar(BAR_V_EMPTY + st));
+          }
+          __syncwarp();
+          // S of the step after the next takes the place of this step's P, once P V has read it: nothing orders products with different
+          // accumulators.  The softmax works on the step between them meanwhile.
+          if (i + 2 < it.steps) ok = wait(BAR_O_DONE + t, g) && issue_s(i + 2);
+        }
+        // the next item's first S take the places of the last two P
+        if (ok) ok = wait(BAR_O_DONE + t, steps + it.steps - 1);
+        steps += it.steps;
+        blocks += stage_of(it, it.steps - 1) + 1;
+        ++full;
+      }
+    } else if (warp == 2) {
+      // ---------------- items ----------------
+      const int cta_rows = p.pair_heads ? BQ : BQ * TILES, cta_heads = p.n_heads / (p.pair_heads ? TILES : 1);
+      const int n_rows = (p.seq + cta_rows - 1) / cta_rows, per_row = p.batch * cta_heads;
+      int next = static_cast<int>(blockIdx.x);
+      for (int k = 0;; ++k) {
+        Item it = {-1, 0, 0, 0, 0};
+        if (next >= 0) {
+          // late queries first: under a causal mask they see the most
+          it.query = (n_rows - 1 - next / per_row) * cta_rows;
+          const int bh = next % per_row;
+          it.batch = bh / cta_heads;
+          it.head = bh % cta_heads * (p.pair_heads ? TILES : 1);
+          const ftb200::KeyRange r = p.mask.keys_of(it.batch, it.query, p.pair_heads ? 1 : TILES, p.seq);
+          it.first = r.lo / SUB;
+          it.steps = r.hi > r.lo ? (r.hi + SUB - 1) / SUB - it.first : 0;
+        }
+        if (!wait(BAR_ITEM_EMPTY + (k & 1), (k >> 1) ^ 1)) break;
+        if (lane == 0) items[k & 1] = it;
+        mbar_arrive_warp(bar(BAR_ITEM_FULL + (k & 1)));
+        if (next < 0 || !wait(BAR_CLAIM, k)) break;
+        if (elect_one()) {
+          mbar_expect_tx(bar(BAR_CLAIMED), 16);
+          claim_next(answer, bar(BAR_CLAIMED));
+        }
+        __syncwarp();
+        if (!wait(BAR_CLAIMED, k)) break;
+        next = claimed(answer);
+        fence_async_smem();  // read before the next answer is written
+        __syncwarp();
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------- softmax + output: one thread per query row ----------------
+    regs_inc<SOFTMAX_REGS>();
+    const int t = (warp - 4) >> 2;   // tile
+    const int quarter = warp & 3;    // TMEM lane quarter this warp may touch
+    const int row = quarter * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t s_addr = tmem_base + C::COL_S + t * 128 + lane_addr;
+    const uint32_t o_addr = tmem_base + C::COL_O + t * D + lane_addr;
+    const uint32_t off_stage = C::OFF_O + (warp - 4) * 4096;
+    uint8_t* stage = smem + off_stage + lane * 128;
+    // with SCORE the scores come scaled, in units of log2
+    const float scale_log2 = SCORE ? 1.f : p.scale_log2;
+    Item it;
+    ftb200::RowMask mine = {0, 0, 0, 0};
+    int steps = 0, full = 0;
+    bool ok = read_item(0, it);
+    if (ok && it.batch >= 0) mine = p.mask.row(it.batch, it.query + t * q_step + row, p.seq);
+    for (int k = 0; ok && it.batch >= 0; ++k) {
+      const int query = it.query + t * q_step + row;
+      const int head = it.head + t * h_step;
+      float slope2 = 0.f;
+      if constexpr (SCORE) slope2 = p.mask.slope2(head);
+      float m_used = -INFINITY, l_sum = 0.f;
+      for (int i = 0; i < it.steps; ++i) {
+        const int g = steps + i;
+        if (!(ok = wait(BAR_S_FULL + 2 * t + (g & 1), g >> 1))) break;
+        tc_fence_after();
+        const uint32_t at = s_addr + (g & 1) * SUB;
+        uint32_t sv[SUB];
+        tmem_ld32(at, sv);
+        tmem_ld32(at + 32, sv + 32);
+        tmem_wait_ld();
+        const int first = (it.first + i) * SUB;
+        if constexpr (SCORE) {
+          p.mask.cap_scores<SUB>(sv);
+          p.mask.slope_scores<SUB>(sv, static_cast<float>(query - first), -1.f, slope2);
+        }
+        if (!mine.all(first, SUB)) {
+#pragma unroll
+          for (int w = 0; w < SUB / 32; ++w) {
+            const uint32_t bits = ftb200::range_bits(mine.lo - first - 32 * w, mine.hi - first - 32 * w);
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (!(bits >> c & 1u)) sv[32 * w + c] = __float_as_uint(-INFINITY);
+          }
+        }
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < SUB; c += 2)
+          mx4[(c >> 1) & 3] = fmaxf(fmaxf(mx4[(c >> 1) & 3], __uint_as_float(sv[c])), __uint_as_float(sv[c + 1]));
+        const float m_new = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+
+        // raise the maximum only when it moved far
+        float alpha = 1.f;
+        const bool raise = i > 0 && (m_new - m_used) * scale_log2 > RESCALE_THRESHOLD;
+        const bool any_raise = __any_sync(0xffffffffu, raise);
+        if (i == 0) {
+          m_used = m_new;
+        } else if (raise) {
+          alpha = exp2f((m_used - m_new) * scale_log2);
+          m_used = m_new;
+          l_sum *= alpha;
+        }
+        if (any_raise) {
+          // O may only be touched once P V of the previous step is done; P V of this step waits for P
+          if (!(ok = wait(BAR_O_DONE + t, g - 1))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t ov[32];
+            tmem_ld32(o_addr + c * 32, ov);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
+            tmem_st32(o_addr + c * 32, ov);
+          }
+        }
+        // a row that has seen nothing yet has no maximum
+        const float neg_m = m_used == -INFINITY ? 0.f : -m_used * scale_log2;
+        const unsigned long long scale2 = f2_pack(scale_log2, scale_log2), neg_m2 = f2_pack(neg_m, neg_m);
+        unsigned long long sum2[2] = {0ull, 0ull};
+#pragma unroll
+        for (int c = 0; c < SUB / 32; ++c) {
+          uint32_t packed[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const unsigned long long x2 =
+                f2_fma(f2_pack(__uint_as_float(sv[c * 32 + 2 * e]), __uint_as_float(sv[c * 32 + 2 * e + 1])), scale2, neg_m2);
+            unsigned long long p2;
+            float p0, p1;
+            if (((e * POLY) & 7) < POLY) {  // POLY of every 8 exponentials go to the FMA pipe
+              p2 = f2_exp2_poly(x2);
+              f2_unpack(p2, p0, p1);
+            } else {
+              f2_unpack(x2, p0, p1);
+              p0 = exp2f(p0);
+              p1 = exp2f(p1);
+              p2 = f2_pack(p0, p1);
+            }
+            sum2[e & 1] = f2_add(sum2[e & 1], p2);
+            __nv_bfloat162 pk = __floats2bfloat162_rn(p0, p1);
+            packed[e] = *reinterpret_cast<uint32_t*>(&pk);
+          }
+          // P replaces the first half of the scores this thread has already taken into registers
+          tmem_st16(at + c * 16, packed);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive_warp(bar(BAR_P_FULL + 2 * t + (g & 1)));
+        float sum4[4];
+        f2_unpack(sum2[0], sum4[0], sum4[1]);
+        f2_unpack(sum2[1], sum4[2], sum4[3]);
+        l_sum += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+      }
+      if (!ok) break;
+      steps += it.steps;
+
+      // the next item's rows are on their way while this one's leave
+      Item next;
+      if (!(ok = read_item(k + 1, next))) break;
+      ftb200::RowMask theirs = {0, 0, 0, 0};
+      if (next.batch >= 0) theirs = p.mask.row(next.batch, next.query + t * q_step + row, p.seq);
+
+      if (it.steps > 0) {
+        if (!(ok = wait(BAR_O_LAST + t, full))) break;
+        ++full;
+      }
+      tc_fence_after();
+      const bool nothing = l_sum == 0.f;  // no key is seen: zeros, and a log-sum-exp of -infinity
+      const float inv = 1.f / l_sum;
+      const int first_row = it.query + t * q_step + quarter * 32;
+      // O leaves by TMA, 32 rows of 64 elements at a time
+#pragma unroll
+      for (int s = 0; s < C::SLABS; ++s) {
+        uint32_t ov[64];
+        tmem_ld32(o_addr + s * 64, ov);
+        tmem_ld32(o_addr + s * 64 + 32, ov + 32);
+        tmem_wait_ld();
+        if (s == C::SLABS - 1 && it.steps > 0) {
+          tc_fence_before();
+          mbar_arrive_warp(bar(BAR_O_FREE + t));
+        }
+        if (lane == 0) bulk_wait_read();  // what was here has left
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          uint32_t u[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float a = nothing ? 0.f : __uint_as_float(ov[8 * c + 2 * e]) * inv, b = nothing ? 0.f : __uint_as_float(ov[8 * c + 2 * e + 1]) * inv;
+            __nv_bfloat162 pk = __floats2bfloat162_rn(a, b);
+            u[e] = *reinterpret_cast<uint32_t*>(&pk);
+          }
+          *reinterpret_cast<uint4*>(stage + ((c ^ (lane & 7)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0 && first_row < p.seq) {
+          tma_store_3d(&tmO, smem_base + off_stage, head * D + s * 64, first_row, it.batch);
+          bulk_commit();
+        }
+        __syncwarp();
+      }
+      if (p.lse != nullptr && query < p.seq) {
+        p.lse[(static_cast<long long>(it.batch) * p.n_heads + head) * p.seq + query] =
+            nothing ? -INFINITY : (m_used * scale_log2 + log2f(l_sum)) * 0.6931471805599453f;
+      }
+      it = next;
+      mine = theirs;
+    }
+    if (lane == 0) bulk_wait_read();
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag && p.status != nullptr) atomicExch(p.status, FTB200_ST_TIMEOUT);
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+  }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* sym = nullptr;
+    cudaDriverEntryPointQueryResult qres;
+    const bool found = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &qres) == cudaSuccess &&
+                       qres == cudaDriverEntryPointSuccess;
+    return found ? reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(sym) : nullptr;
+  }();
+  return fn;
+}
+
+// [batch, seq, cols] bf16 view with row stride ld (elements); box = 64 columns x box_rows, 128-byte swizzle
+int encode_rows(CUtensorMap* map, const void* base, long long batch, long long seq, long long cols, long long ld, unsigned box_rows) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return FTB200_E_DRIVER;
+  cuuint64_t gdim[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(seq), static_cast<cuuint64_t>(batch)};
+  cuuint64_t gstride[2] = {static_cast<cuuint64_t>(ld) * 2, static_cast<cuuint64_t>(seq) * ld * 2};
+  cuuint32_t box[3] = {64u, box_rows, 1u};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : FTB200_E_DRIVER;
+}
+
+struct Maps {
+  CUtensorMap q, k, v, o;
+};
+
+template <int D, int POLY, bool SCORE>
+int launch(const Maps& m, const Params& p, long long grid, cudaStream_t stream) {
+  auto* kernel = attention_masked_fwd_kernel<D, POLY, SCORE>;
+  static std::atomic<unsigned long long> ready{0};  // per device
+  if (!ftb200::once_per_device(ready)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM_BYTES) != cudaSuccess) return FTB200_E_CUDA;
+    // The warpgroups' register split assumes this count, which the compiler gives a kernel that moves registers; with fewer the softmax
+    // warpgroups would wait for registers that nobody has.
+    cudaFuncAttributes attr;
+    if (cudaFuncGetAttributes(&attr, kernel) != cudaSuccess) return FTB200_E_CUDA;
+    if (attr.numRegs < LAUNCH_REGS) return FTB200_E_REGS;
+    ftb200::done_on_device(ready);
+  }
+  ftb200::launch_after(kernel, static_cast<unsigned>(grid), NUM_THREADS, Cfg<D>::SMEM_BYTES, stream, m.q, m.k, m.v, m.o, p);
+  return cudaGetLastError() == cudaSuccess ? 0 : FTB200_E_CUDA;
+}
+
+}  // namespace
+
+// q: [batch*seq, n_heads*head_dim] view with row stride ld_q; k, v: [batch*seq, n_kv_heads*head_dim] views with row strides ld_k, ld_v; o:
+// [batch*seq, n_heads*head_dim] with row stride ld_o.  lse (may be null): [batch, n_heads, seq] fp32.  head_dim 64 or 128, any seq.
+// rows, tiles, padded: null, where every query sees the keys up to its own (causal) or all, or what ftb200_attention_spans wrote.
+// softcap: 0, or what the scores are capped at, softcap tanh(scale s / softcap).  slopes: null, or [n_heads] fp32: slope |query - key| is
+// subtracted from a score.
+FTB200_API int ftb200_attention_masked_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const void* rows, const void* tiles,
+                                           const int* padded, const float* slopes, int batch, int seq, int n_heads, int n_kv_heads, int head_dim,
+                                           long long ld_q, long long ld_k, long long ld_v, long long ld_o, float scale, float softcap, int causal,
+                                           int* status, cudaStream_t stream) {
+  if ((head_dim != 64 && head_dim != 128) || batch <= 0 || seq <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0)
+    return FTB200_E_BADARG;
+  for (const void* x : {q, k, v, (const void*)o})
+    if (reinterpret_cast<uintptr_t>(x) & 15) return FTB200_E_ALIGN;
+  for (long long x : {ld_q, ld_k, ld_v, ld_o})
+    if (x & 7) return FTB200_E_ALIGN;
+  Params p = {};
+  Maps m;
+  int rc = ftb200::set_mask(&p.mask, rows, tiles, padded, slopes, scale, softcap, causal, seq);
+  if (rc == 0) rc = encode_rows(&m.q, q, batch, seq, static_cast<long long>(n_heads) * head_dim, ld_q, 128);
+  if (rc == 0) rc = encode_rows(&m.k, k, batch, seq, static_cast<long long>(n_kv_heads) * head_dim, ld_k, 128);
+  if (rc == 0) rc = encode_rows(&m.v, v, batch, seq, static_cast<long long>(n_kv_heads) * head_dim, ld_v, 128);
+  if (rc == 0) rc = encode_rows(&m.o, o, batch, seq, static_cast<long long>(n_heads) * head_dim, ld_o, 32);
+  if (rc != 0) return rc;
+  p.batch = batch; p.seq = seq; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.lse = lse; p.status = status;
+  p.pair_heads = n_heads / n_kv_heads % TILES == 0;
+  const long long tiles_q = (static_cast<long long>(seq) + BQ - 1) / BQ;
+  const long long grid = p.pair_heads ? batch * (static_cast<long long>(n_heads) / TILES) * tiles_q
+                                      : static_cast<long long>(batch) * n_heads * ((tiles_q + TILES - 1) / TILES);
+  if (grid > 0x7fffffffLL) return FTB200_E_TOOBIG;
+  const bool score = softcap > 0.f || slopes != nullptr;
+  if (head_dim == 128) return score ? launch<128, 0, true>(m, p, grid, stream) : launch<128, 0, false>(m, p, grid, stream);
+  return score ? launch<64, 0, true>(m, p, grid, stream) : launch<64, 2, false>(m, p, grid, stream);
+}

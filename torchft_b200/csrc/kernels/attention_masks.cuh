@@ -8,10 +8,10 @@
 //
 //   y = log2(e) (softcap tanh(scale s / softcap) - slope |query - key|)
 //
-// tanh(x) is x P(x^2) up to |x| = 0.8, where P of degree 5 has a relative error of 5.8e-8 (least largest error, by Lawson's iteration of weighted
-// least squares): seven operations of the FMA pipe, with scale and cap inside the coefficients, while the exponential unit, which the softmax
-// wants for itself, stays free.  A thread's scores that go beyond take 1 - 2 / (exp(2x) + 1), with an error of about 1e-7 of the cap, which
-// is what counts in a score.
+// tanh(x) is x P(x^2), of degree 3 up to |x| = 0.4 (a relative error of 9.8e-8) and of degree 5 up to 0.8 (5.8e-8; least largest error, by
+// Lawson's iteration of weighted least squares): five or seven operations of the FMA pipe, with scale and cap inside the coefficients, while the
+// exponential unit, which the softmax wants for itself, stays free.  A warp's scores that go beyond take 1 - 2 / (exp(2x) + 1), with an error
+// of about 1e-7 of the cap, which is what counts in a score.
 #pragma once
 
 #include <limits.h>
@@ -47,8 +47,8 @@ struct MaskParams {
   int capped;
   const float* slopes;  // null, or [heads]
   float scale_log2;     // log2(e) scale
-  float poly[6];        // of s^2: y = s P(s^2)
-  float poly_up_to;     // |s| that it holds for
+  float near[4], poly[6];  // of s^2: y = s P(s^2)
+  float near_up_to, poly_up_to;  // |s| that they hold for
   float cap2;           // log2(e) softcap
   float in2;            // 2 log2(e) scale / softcap
   float neg_inv_cap2_sq;  // -1 / cap2^2: 1 - tanh^2 = 1 + y^2 times this
@@ -132,6 +132,26 @@ struct MaskParams {
 
   __device__ __forceinline__ float slope2(int head) const { return slopes == nullptr ? 0.f : slopes[head] * 1.4426950408889634f; }
 
+  template <int N, int K>
+  static __device__ __forceinline__ void by_polynomial(uint32_t* sv, const float* coefficients) {
+    using namespace tc;
+    unsigned long long k[K];
+#pragma unroll
+    for (int i = 0; i < K; ++i) k[i] = f2_pack(coefficients[i], coefficients[i]);
+#pragma unroll
+    for (int c = 0; c < N; c += 2) {
+      const unsigned long long s = f2_pack(__uint_as_float(sv[c]), __uint_as_float(sv[c + 1]));
+      const unsigned long long u = f2_mul(s, s);
+      unsigned long long y = f2_fma(u, k[K - 1], k[K - 2]);
+#pragma unroll
+      for (int i = K - 3; i >= 0; --i) y = f2_fma(u, y, k[i]);
+      float y0, y1;
+      f2_unpack(f2_mul(s, y), y0, y1);
+      sv[c] = __float_as_uint(y0);
+      sv[c + 1] = __float_as_uint(y1);
+    }
+  }
+
   // A thread's N products become log2(e) softcap tanh(scale s / softcap), or log2(e) scale s without a cap.
   template <int N>
   __device__ __forceinline__ void cap_scores(uint32_t* sv) const {
@@ -141,22 +161,11 @@ struct MaskParams {
 #pragma unroll
       for (int c = 0; c < N; c += 2)
         big[(c >> 1) & 3] = fmaxf(fmaxf(big[(c >> 1) & 3], fabsf(__uint_as_float(sv[c]))), fabsf(__uint_as_float(sv[c + 1])));
-      if (__all_sync(0xffffffffu, fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) <= poly_up_to)) {
-        unsigned long long k[6];
-#pragma unroll
-        for (int i = 0; i < 6; ++i) k[i] = f2_pack(poly[i], poly[i]);
-#pragma unroll
-        for (int c = 0; c < N; c += 2) {
-          const unsigned long long s = f2_pack(__uint_as_float(sv[c]), __uint_as_float(sv[c + 1]));
-          const unsigned long long u = f2_mul(s, s);
-          unsigned long long y = f2_fma(u, k[5], k[4]);
-#pragma unroll
-          for (int i = 3; i >= 0; --i) y = f2_fma(u, y, k[i]);
-          float y0, y1;
-          f2_unpack(f2_mul(s, y), y0, y1);
-          sv[c] = __float_as_uint(y0);
-          sv[c + 1] = __float_as_uint(y1);
-        }
+      const float most = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
+      if (__all_sync(0xffffffffu, most <= near_up_to)) {
+        by_polynomial<N, 4>(sv, near);
+      } else if (__all_sync(0xffffffffu, most <= poly_up_to)) {
+        by_polynomial<N, 6>(sv, poly);
       } else {
 #pragma unroll
         for (int c = 0; c < N; ++c) {
@@ -196,13 +205,16 @@ inline int set_mask(MaskParams* m, const void* rows, const void* tiles, const in
   if (softcap > 0.f) {
     constexpr double P[6] = {0.9999999420836679, -0.333326749210523, 0.1332104829082429, -0.05311431573861419, 0.01909330062970014,
                              -0.004355299563624438};
+    constexpr double NEAR[4] = {0.9999999019017232, -0.33331362461616354, 0.132709767765151, -0.04755360368917723};
     const double k = static_cast<double>(scale) / softcap, cap2 = softcap * LOG2E;
     double power = cap2 * k;
     bool fits = true;
     for (int i = 0; i < 6; ++i, power *= k * k) {
+      if (i < 4) m->near[i] = static_cast<float>(NEAR[i] * power);
       m->poly[i] = static_cast<float>(P[i] * power);
       fits = fits && isfinite(m->poly[i]);
     }
+    m->near_up_to = fits ? static_cast<float>(0.4 / k) : -1.f;
     m->poly_up_to = fits ? static_cast<float>(0.8 / k) : -1.f;
     m->cap2 = static_cast<float>(cap2);
     m->in2 = static_cast<float>(2.0 * LOG2E * k);

@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(ROPE_THREADS, 4) rope_axes_kernel(T* buf, cons
       if (w.token >= n_tokens) break;
       const T* p = address(w);
 #pragma unroll
-      for (int e = 0; e < VECS; ++e) x[k][e] = *reinterpret_cast<const V*>(p + e * half);
+      for (int e = 0; e < VECS; ++e) *reinterpret_cast<uint4*>(&x[k][e]) = *reinterpret_cast<const uint4*>(p + e * half);
     }
   };
   load(at);
@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(ROPE_THREADS, 4) rope_axes_kernel(T* buf, cons
         }
       }
 #pragma unroll
-      for (int e = 0; e < VECS; ++e) *reinterpret_cast<V*>(p + e * half) = x[k][e];
+      for (int e = 0; e < VECS; ++e) *reinterpret_cast<uint4*>(p + e * half) = *reinterpret_cast<const uint4*>(&x[k][e]);
     }
     load(at);
   }
