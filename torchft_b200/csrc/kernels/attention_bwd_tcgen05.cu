@@ -347,7 +347,7 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       const bool padded = MASK && p.mask.has_padding(b, p.seq, lane);
       TileWalk next{h0, first_q};  // the tile whose Q or dO is waited for
       auto clear = [&](uint32_t off, int tile) {
-        if (padded) p.mask.clear_padding(smem + off, SLABS, b, tile, p.seq, lane);
+        if (padded) p.mask.clear_padding(smem + off, SLABS, b, tile * 128, p.seq, lane);
       };
       bool ok = (!MASK || T > 0) && wait(BAR_KV, 0) && wait(BAR_Q_FULL, 0);
       if (ok) {

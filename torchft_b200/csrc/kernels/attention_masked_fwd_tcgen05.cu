@@ -6,25 +6,25 @@
 // [batch * seq, n_cols] activation (any row stride).
 //
 // An item of work is one (batch, pair of tiles of 128 queries): two heads of a group at the same queries where the group's size is even, so that
-// the tiles look at the same keys, and two query tiles of a head otherwise.  Both walk over the 64-key blocks that some query of them sees.
-// Documents make items short (8 blocks of 128 keys where 1000 tokens are a document) and unequal, so what surrounds them counts as much as
-// their loop:
+// the tiles look at the same keys, and two query tiles of a head otherwise.  Both walk over blocks of 128 keys, from the first key that some query
+// of them sees on.  Documents make items short (8 blocks where 1000 tokens are a document) and unequal, so what surrounds them counts as much
+// as their loop: a CTA per SM stays and takes items one after another, in the grid's order, by cancelling CTAs that have not been launched yet
+// (cluster launch control), the next one when its current item is nearly done.  The next item's Q, K and first product are under way while
+// the current one's output leaves.  As a CTA of its own an item of one block took 8.6 us, of which 1.4 in the softmax.
 //
-//   - a CTA per SM stays and takes items one after another, in the grid's order, by cancelling CTAs that have not been launched yet (cluster
-//     launch control), the next one when its current item is nearly done; the next item's Q, K and first products are under way while the
-//     current one's output leaves.  As a CTA of its own an item of one key block took 8.6 us, of which 1.4 in the softmax;
-//   - the scores of a tile have two buffers of 64 keys each, so that a block's product S = Q K^T runs while the softmax works on the one
-//     before: with one buffer of 128 keys the softmax waited 1224 of 3552 cycles for P V and the next S;
-//   - blocks that each query sees need no mask; in the others a row's seen keys are a run of bits.
-//
-//   warp 0        TMA: Q tiles of an item, K and V blocks of 128 keys into a 2-stage ring
-//   warps 1, 3    tcgen05.mma of a tile each, per block of 64 keys: P V, then S of the block after the next.  (One warp for both spent
-//                 220 cycles and more on every wait, beside two softmax warps, and was what bounded the loop.)
+//   warp 0        TMA: Q tiles of an item, K and V blocks into a ring
+//   warp 1        tcgen05.mma, in the order P0 V, S0', P1 V, S1' (' = next block): the softmax of a tile has the other's products to hide
+//                 under.  (A warp for each tile lets the tiles fall into step: 4480 cycles for two tiles' 128 keys instead of 3630.)
 //   warp 2        the next item: launch control, the range of its keys
-//   warps 4..7    softmax and output of tile 0, warps 8..11 of tile 1: one thread per query row
+//   warps 4..7    softmax and output of tile 0, warps 8..11 of tile 1: one thread per query row.  (Four lanes a row in sixteen warps, two rows of
+//                 32 scores a thread, are 16 % faster at head dim 64 and 7 % slower at 128.)
 //
-// The running maximum is only raised (and O in TMEM rescaled) when it grows by more than 2^8.  P goes back as packed bf16 into the first 32
-// columns of the scores it came from and is the A operand of P V straight from tensor memory.
+// P goes back as packed bf16 and is the A operand of P V straight from tensor memory, of its first half while the exponentials of the second are
+// computed.  At head dim 64 it has columns of its own, so that S of the next block runs under this one's softmax; at head dim 128 the 512
+// columns are full (two S, two O) and it takes the place of the scores that it came from.  (Scores in two buffers of 64 keys instead read Q
+// twice as often from shared memory: 4900 cycles.)
+// The running maximum is only raised (and O in TMEM rescaled) when it grows by more than 2^8.  Blocks that each query sees need no mask; in the
+// others a row's seen keys are a run of bits.
 //
 // Sequences of any length: the tensor maps have the sequence as a dimension of its own, so a tile's rows beyond its end are zeros (not the
 // next sequence's); keys there are in no query's range, queries there are not stored.
@@ -44,17 +44,15 @@ using namespace ftb200::tc;
 
 constexpr int BQ = 128;    // queries per tile
 constexpr int TILES = 2;   // tiles per item
-constexpr int BKV = 128;   // keys per stage of K and V
-constexpr int SUB = 64;    // keys per step of the softmax
-constexpr int STAGES = 2;  // of K and V, of the scores, and of the items
+constexpr int BKV = 128;   // keys per block
 constexpr int NUM_THREADS = 384;
 // Registers: a CTA is launched with 168 a thread (65536 / 384, checked on the host); the first warpgroup gives most of its own to the two
 // softmax warpgroups: 72 + 2 * 216 = 3 * 168.
 constexpr int LAUNCH_REGS = 168, ISSUE_REGS = 72, SOFTMAX_REGS = 216;
 static_assert(ISSUE_REGS + 2 * SOFTMAX_REGS <= 3 * LAUNCH_REGS, "more registers than the CTA is launched with");
 constexpr int ROW_WARPS = 4;                  // softmax warps per tile
-constexpr int READERS = 1 + TILES + TILES * ROW_WARPS;  // warps that read an item
-constexpr int CLAIM_AHEAD = 6;                // steps before its end at which an item asks for the next one
+constexpr int READERS = 2 + TILES * ROW_WARPS;  // warps that read an item
+constexpr int CLAIM_AHEAD = 3;                // blocks before its end at which an item asks for the next one
 constexpr uint32_t TMEM_COLS = 512;
 constexpr float RESCALE_THRESHOLD = 8.0f;  // in log2 units
 
@@ -63,14 +61,17 @@ struct Cfg {
   static constexpr uint32_t TILE_BYTES = 128 * D * 2;  // a 128-row operand tile
   static constexpr uint32_t SLAB_BYTES = 128 * 128;    // 128 rows x 64 elements (one swizzle atom wide)
   static constexpr int SLABS = D / 64;
+  static constexpr int STAGES = D == 128 ? 2 : 4;  // of K and V
+  static constexpr bool OWN_P = D == 64;           // P has columns of its own
   static constexpr uint32_t OFF_Q = 0;                    // Q0 Q1
-  static constexpr uint32_t OFF_KV = TILES * TILE_BYTES;  // K0 V0 | K1 V1
+  static constexpr uint32_t OFF_KV = TILES * TILE_BYTES;  // K0 V0 | K1 V1 | ...
   static constexpr uint32_t OFF_O = OFF_KV + STAGES * 2 * TILE_BYTES;  // per softmax warp: 32 rows x 64 elements on their way out
   static constexpr uint32_t OFF_MISC = OFF_O + TILES * ROW_WARPS * 4096;
   static constexpr uint32_t SMEM_BYTES = OFF_MISC + 512 + 1024;
   static_assert(SMEM_BYTES <= 232448, "exceeds the 227 KB of shared memory a CTA can have");
-  static constexpr uint32_t COL_S = 0;    // S of tile t, buffer s at COL_S + t * 128 + s * 64
+  static constexpr uint32_t COL_S = 0;    // S_t at COL_S + t * 128
   static constexpr uint32_t COL_O = 256;  // O_t at COL_O + t * D
+  static constexpr uint32_t COL_P = OWN_P ? 384 : COL_S, P_STEP = OWN_P ? 64 : 128;  // P_t at COL_P + t * P_STEP
 };
 
 struct Params {
@@ -85,26 +86,29 @@ struct Params {
 struct Item {
   int batch;  // below zero: there is none
   int head, query;
-  int first, steps;  // blocks of 64 keys
+  int first, blocks;  // key of the first block, number of blocks
+  int all_lo[TILES], all_hi[TILES];  // keys that each query of the tile sees
 };
 
 enum : int {
-  BAR_Q_FULL = 0,     // +tile
-  BAR_Q_EMPTY = 2,    // +tile
-  BAR_K_FULL = 4,     // +stage
-  BAR_K_EMPTY = 6,    // +stage
-  BAR_V_FULL = 8,     // +stage
-  BAR_V_EMPTY = 10,   // +stage
-  BAR_S_FULL = 12,    // +2 tile + buffer
-  BAR_P_FULL = 16,    // +2 tile + buffer
-  BAR_O_DONE = 20,    // +tile: P V of a step
-  BAR_O_FREE = 22,    // +tile: O has been read
-  BAR_ITEM_FULL = 24,   // +slot
-  BAR_ITEM_EMPTY = 26,  // +slot
-  BAR_CLAIM = 28,     // the current item is nearly done
-  BAR_CLAIMED = 29,   // the answer of the launch control
-  BAR_O_LAST = 30,    // +tile: P V of an item's last step (who waits for it may be two steps behind, which a parity does not tell apart)
-  NUM_BARS = 32,
+  BAR_Q_FULL = 0,    // +tile
+  BAR_Q_EMPTY = 2,   // +tile
+  BAR_K_FULL = 4,    // +stage
+  BAR_K_EMPTY = 8,   // +stage
+  BAR_V_FULL = 12,   // +stage
+  BAR_V_EMPTY = 16,  // +stage
+  BAR_S_FULL = 20,   // +tile
+  BAR_S_READ = 22,   // +tile: the scores are in registers (where P has columns of its own)
+  BAR_P_HALF = 24,   // +tile: P of the block's first 64 keys
+  BAR_P_FULL = 26,   // +tile
+  BAR_O_DONE = 28,   // +tile: P V of a block
+  BAR_O_LAST = 30,   // +tile: P V of an item's last block
+  BAR_O_FREE = 32,   // +tile: O has been read
+  BAR_ITEM_FULL = 34,   // +slot
+  BAR_ITEM_EMPTY = 36,  // +slot
+  BAR_CLAIM = 38,    // the current item is nearly done
+  BAR_CLAIMED = 39,  // the answer of the launch control
+  NUM_BARS = 40,
 };
 
 // The grid's next CTA that has not been launched, or -1: the answer (16 bytes) arrives in shared memory with the barrier.
@@ -137,16 +141,16 @@ attention_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_MISC);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC + 256);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 260);
-  Item* items = reinterpret_cast<Item*>(smem + C::OFF_MISC + 288);  // two slots
-  static_assert(NUM_BARS * 8 <= 256 && 288 + 2 * sizeof(Item) <= 384, "barriers, slots and the answer overlap");
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC + 320);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 324);
+  Item* items = reinterpret_cast<Item*>(smem + C::OFF_MISC + 336);  // two slots
+  static_assert(NUM_BARS * 8 <= 320 && 336 + 2 * sizeof(Item) <= 448, "barriers, slots and the answer overlap");
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
   const uint32_t smem_base = smem_u32(smem);
   const uint32_t bar_base = smem_u32(bars);
-  const uint32_t answer = smem_base + C::OFF_MISC + 384;
+  const uint32_t answer = smem_base + C::OFF_MISC + 448;
   auto bar = [&](int i) { return bar_base + 8u * i; };
   auto wait = [&](int which, uint32_t parity) { return mbar_wait_warp(bar(which), parity & 1u, abort_flag); };
 
@@ -157,21 +161,21 @@ attention_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
     for (int t = 0; t < TILES; ++t) {
       mbar_init(bar(BAR_Q_FULL + t), 1);
       mbar_init(bar(BAR_Q_EMPTY + t), 1);
+      mbar_init(bar(BAR_S_FULL + t), 1);
+      mbar_init(bar(BAR_S_READ + t), ROW_WARPS);
+      mbar_init(bar(BAR_P_HALF + t), ROW_WARPS);
+      mbar_init(bar(BAR_P_FULL + t), ROW_WARPS);
       mbar_init(bar(BAR_O_DONE + t), 1);
       mbar_init(bar(BAR_O_LAST + t), 1);
       mbar_init(bar(BAR_O_FREE + t), ROW_WARPS);
-      for (int s = 0; s < STAGES; ++s) {
-        mbar_init(bar(BAR_S_FULL + 2 * t + s), 1);
-        mbar_init(bar(BAR_P_FULL + 2 * t + s), ROW_WARPS);
-      }
+      mbar_init(bar(BAR_ITEM_FULL + t), 1);  // two slots
+      mbar_init(bar(BAR_ITEM_EMPTY + t), READERS);
     }
-    for (int s = 0; s < STAGES; ++s) {
+    for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(bar(BAR_K_FULL + s), 1);
-      mbar_init(bar(BAR_K_EMPTY + s), TILES);
+      mbar_init(bar(BAR_K_EMPTY + s), 1);
       mbar_init(bar(BAR_V_FULL + s), 1);
-      mbar_init(bar(BAR_V_EMPTY + s), TILES);
-      mbar_init(bar(BAR_ITEM_FULL + s), 1);
-      mbar_init(bar(BAR_ITEM_EMPTY + s), READERS);
+      mbar_init(bar(BAR_V_EMPTY + s), 1);
     }
     mbar_init(bar(BAR_CLAIM), 1);
     mbar_init(bar(BAR_CLAIMED), 1);
@@ -194,15 +198,10 @@ attention_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
   auto read_item = [&](int k, Item& it) {
     if (!wait(BAR_ITEM_FULL + (k & 1), k >> 1)) return false;
     const Item& at = items[k & 1];
-    // from lane 0, so that what depends on it, the MMAs' descriptors above all, is known to be the same in all lanes and stays in uniform registers
-    auto same = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
-    it = {same(at.batch), same(at.head), same(at.query), same(at.first), same(at.steps)};
+    it = at;
     mbar_arrive_warp(bar(BAR_ITEM_EMPTY + (k & 1)));
     return true;
   };
-  // the stage of K and V that step i lies in, counted from the item's first
-  auto stage_of = [](const Item& it, int i) { return ((it.first + i) >> 1) - (it.first >> 1); };
-
   if (warp < 4) {
     regs_dec<ISSUE_REGS>();
     if (warp == 0) {
@@ -212,49 +211,29 @@ attention_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
       for (int k = 0; ok; ++k) {
         Item it;
         if (!(ok = read_item(k, it)) || it.batch < 0) break;
-        if (it.steps == 0) continue;
+        if (it.blocks == 0) continue;
         const int hk = it.head / rep;
-        for (int t = 0; t < TILES && ok; ++t) {
-          if (!(ok = wait(BAR_Q_EMPTY + t, full ^ 1))) break;
+        auto load = [&](const CUtensorMap* map, int full_bar, uint32_t dst, int col, int r) {
           if (elect_one()) {
-            const uint32_t sq = smem_base + C::OFF_Q + t * C::TILE_BYTES;
-            mbar_expect_tx(bar(BAR_Q_FULL + t), C::TILE_BYTES);
-            for (int s = 0; s < C::SLABS; ++s)
-              tma_load_3d(sq + s * C::SLAB_BYTES, &tmQ, bar(BAR_Q_FULL + t), (it.head + t * h_step) * D + s * 64, it.query + t * q_step, it.batch);
+            mbar_expect_tx(bar(full_bar), C::TILE_BYTES);
+            for (int s = 0; s < C::SLABS; ++s) tma_load_3d(dst + s * C::SLAB_BYTES, map, bar(full_bar), col * D + s * 64, r, it.batch);
           }
           __syncwarp();
-          if (t > 0) break;
-          // the first block of keys between the two
-          const int st = blocks & 1;
-          if (!(ok = wait(BAR_K_EMPTY + st, (blocks >> 1) ^ 1))) break;
-          if (elect_one()) {
-            const uint32_t sk = smem_base + C::OFF_KV + st * 2 * C::TILE_BYTES;
-            mbar_expect_tx(bar(BAR_K_FULL + st), C::TILE_BYTES);
-            for (int s = 0; s < C::SLABS; ++s)
-              tma_load_3d(sk + s * C::SLAB_BYTES, &tmK, bar(BAR_K_FULL + st), hk * D + s * 64, (it.first >> 1) * BKV, it.batch);
-          }
-          __syncwarp();
-        }
-        const int n = stage_of(it, it.steps - 1) + 1;
-        for (int j = 0; j < n && ok; ++j, ++blocks) {
-          const int st = blocks & 1, use = blocks >> 1;
+        };
+        auto load_q = [&](int t) {
+          if (!wait(BAR_Q_EMPTY + t, full ^ 1)) return false;
+          load(&tmQ, BAR_Q_FULL + t, smem_base + C::OFF_Q + t * C::TILE_BYTES, it.head + t * h_step, it.query + t * q_step);
+          return true;
+        };
+        ok = load_q(0);
+        for (int j = 0; j < it.blocks && ok; ++j, ++blocks) {
+          const int st = blocks % C::STAGES, use = blocks / C::STAGES;
           const uint32_t sk = smem_base + C::OFF_KV + st * 2 * C::TILE_BYTES;
-          const int key = ((it.first >> 1) + j) * BKV;
-          if (j > 0) {
-            if (!(ok = wait(BAR_K_EMPTY + st, use ^ 1))) break;
-            if (elect_one()) {
-              mbar_expect_tx(bar(BAR_K_FULL + st), C::TILE_BYTES);
-              for (int s = 0; s < C::SLABS; ++s) tma_load_3d(sk + s * C::SLAB_BYTES, &tmK, bar(BAR_K_FULL + st), hk * D + s * 64, key, it.batch);
-            }
-            __syncwarp();
-          }
+          if (!(ok = wait(BAR_K_EMPTY + st, use ^ 1))) break;
+          load(&tmK, BAR_K_FULL + st, sk, hk, it.first + j * BKV);
+          if (j == 0 && !(ok = load_q(1))) break;
           if (!(ok = wait(BAR_V_EMPTY + st, use ^ 1))) break;
-          if (elect_one()) {
-            mbar_expect_tx(bar(BAR_V_FULL + st), C::TILE_BYTES);
-            for (int s = 0; s < C::SLABS; ++s)
-              tma_load_3d(sk + C::TILE_BYTES + s * C::SLAB_BYTES, &tmV, bar(BAR_V_FULL + st), hk * D + s * 64, key, it.batch);
-          }
-          __syncwarp();
+          load(&tmV, BAR_V_FULL + st, sk + C::TILE_BYTES, hk, it.first + j * BKV);
         }
         ++full;
       }
@@ -264,94 +243,104 @@ attention_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
         const uint64_t t0 = ftb200::globaltimer_ns();
         while (ftb200::globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
       }
-    } else if (warp != 2) {
-      // ---------------- MMA issuers: warp 1 for tile 0, warp 3 for tile 1 ----------------
-      const int t = warp >> 1;
-      // S = Q K^T: both operands K-major (head dim contiguous), M = 128, N = 64
+    } else if (warp == 1) {
+      // ---------------- MMA issuer ----------------
+      // S = Q K^T: both operands K-major (head dim contiguous), M = N = 128
       const uint32_t F = (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(BQ >> 4) << 24);
-      const uint32_t idesc_s = F | (static_cast<uint32_t>(SUB >> 3) << 17);
+      const uint32_t idesc_s = F | (static_cast<uint32_t>(BKV >> 3) << 17);
       // O += P V: A = P from tensor memory (keys contiguous), B = V MN-major (stored [key][d]), N = D
       const uint32_t idesc_o = F | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17);
       constexpr uint32_t HI = smem_desc_hi(1024);
-      constexpr uint32_t HALF16 = (SUB * 128) >> 4;  // the second 64 keys of a stage
-      const uint32_t q_lo = smem_desc_lo(smem_base + C::OFF_Q + t * C::TILE_BYTES, 16);
+      const uint32_t q_lo = smem_desc_lo(smem_base + C::OFF_Q, 16);
       const uint32_t k_lo = smem_desc_lo(smem_base + C::OFF_KV, 16);
       const uint32_t v_lo = smem_desc_lo(smem_base + C::OFF_KV + C::TILE_BYTES, C::SLAB_BYTES);
-      constexpr uint32_t STAGE16 = (2 * C::TILE_BYTES) >> 4;
+      constexpr uint32_t STAGE16 = (2 * C::TILE_BYTES) >> 4, QTILE16 = C::TILE_BYTES >> 4;
+      // taken from lane 0 where it is used, so that it is known to be the same in all lanes and lies in uniform registers
+      auto same = [](uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); };
       bool ok = true;
-      int steps = 0, blocks = 0, full = 0;
+      int blocks = 0, full = 0;
       for (int k = 0; ok; ++k) {
         Item it;
         if (!(ok = read_item(k, it)) || it.batch < 0) break;
-        if (it.steps == 0) {
-          if (t == 0 && elect_one()) mbar_arrive(bar(BAR_CLAIM));
+        if (it.blocks == 0) {
+          if (elect_one()) mbar_arrive(bar(BAR_CLAIM));
           __syncwarp();
           continue;
         }
         const bool padded = p.mask.has_padding(it.batch, p.seq, lane);
         // what stands in padding reaches neither the products nor the choice of a way for the scores
-        auto clear = [&](uint32_t off, int row) {
-          if (padded && row < p.seq) p.mask.clear_padding(smem + off, C::SLABS, it.batch, row / 128, p.seq, lane);
+        auto clear = [&](uint32_t off, int r) {
+          if (padded) p.mask.clear_padding(smem + off, C::SLABS, it.batch, r, p.seq, lane);
         };
-        auto opens = [&](int i) { return i == 0 || ((it.first + i) & 1) == 0; };
-        auto closes = [&](int i) { return i == it.steps - 1 || ((it.first + i) & 1) != 0; };
-        auto issue_s = [&](int i) {
-          const int g = steps + i, blk = blocks + stage_of(it, i), st = blk & 1;
-          if (opens(i)) {
-            if (!wait(BAR_K_FULL + st, blk >> 1)) return false;
-            clear(C::OFF_KV + st * 2 * C::TILE_BYTES, ((it.first + i) >> 1) * BKV);
+        auto issue_s = [&](int t, int j) {
+          const int g = blocks + j, st = g % C::STAGES;
+          if (t == 0) {
+            if (!wait(BAR_K_FULL + st, g / C::STAGES)) return false;
+            clear(C::OFF_KV + st * 2 * C::TILE_BYTES, it.first + j * BKV);
           }
+          if (j == 0) {
+            if (!wait(BAR_Q_FULL + t, full)) return false;
+            clear(C::OFF_Q + t * C::TILE_BYTES, it.query + t * q_step);
+          }
+          // where P is elsewhere the scores of the block before have to be in registers
+          if (C::OWN_P && g > 0 && !wait(BAR_S_READ + t, g - 1)) return false;
           tc_fence_after();
-          const uint32_t kb = k_lo + st * STAGE16 + ((it.first + i) & 1) * HALF16;
-          const uint32_t d_tmem = tmem_base + C::COL_S + t * 128 + (g & 1) * SUB;
+          const uint32_t kb = same(k_lo + st * STAGE16);
           if (elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
               const uint32_t off = ((kk >> 2) * C::SLAB_BYTES + (kk & 3) * 32) >> 4;
-              umma_bf16_lh(d_tmem, q_lo + off, HI, kb + off, HI, idesc_s, kk != 0);
+              umma_bf16_lh(tmem_base + C::COL_S + t * 128, q_lo + t * QTILE16 + off, HI, kb + off, HI, idesc_s, kk != 0);
             }
-            umma_commit(bar(BAR_S_FULL + 2 * t + (g & 1)));
-            if (i == it.steps - 1) umma_commit(bar(BAR_Q_EMPTY + t));
-            if (closes(i)) umma_commit(bar(BAR_K_EMPTY + st));
+            umma_commit(bar(BAR_S_FULL + t));
+            if (t == 1) umma_commit(bar(BAR_K_EMPTY + st));
+            if (j == it.blocks - 1) umma_commit(bar(BAR_Q_EMPTY + t));
           }
           __syncwarp();
           return true;
         };
-        if (!(ok = wait(BAR_Q_FULL + t, full))) break;
-        clear(C::OFF_Q + t * C::TILE_BYTES, it.query + t * q_step);
-        ok = issue_s(0) && (it.steps == 1 || issue_s(1));
-        for (int i = 0; i < it.steps && ok; ++i) {
-          if (t == 0 && i == max(0, it.steps - CLAIM_AHEAD)) {
+        auto issue_pv = [&](int t, int j) {
+          const int g = blocks + j, st = g % C::STAGES;
+          if (t == 0) {
+            if (!wait(BAR_V_FULL + st, g / C::STAGES)) return false;
+            clear(C::OFF_KV + st * 2 * C::TILE_BYTES + C::TILE_BYTES, it.first + j * BKV);
+          }
+          if (j == 0 && full > 0 && !wait(BAR_O_FREE + t, full - 1)) return false;
+          const uint32_t vb = same(v_lo + st * STAGE16);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if (!wait((half == 0 ? BAR_P_HALF : BAR_P_FULL) + t, g)) return false;
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = half * 4; kk < half * 4 + 4; ++kk)  // P: keys 2k, 2k+1 in column k
+                umma_bf16_tmem_a(tmem_base + C::COL_O + t * D, tmem_base + C::COL_P + t * C::P_STEP + kk * 8, vb + ((kk * 2048) >> 4), HI, idesc_o,
+                                 (j | kk) != 0);
+              if (half == 1) {
+                umma_commit(bar(BAR_O_DONE + t));
+                if (t == 1) umma_commit(bar(BAR_V_EMPTY + st));
+                if (j == it.blocks - 1) umma_commit(bar(BAR_O_LAST + t));
+              }
+            }
+            __syncwarp();
+          }
+          return true;
+        };
+        ok = issue_s(0, 0) && issue_s(1, 0);
+        for (int j = 0; j < it.blocks && ok; ++j) {
+          if (j == max(0, it.blocks - CLAIM_AHEAD)) {
             if (elect_one()) mbar_arrive(bar(BAR_CLAIM));
             __syncwarp();
           }
-          const int g = steps + i, blk = blocks + stage_of(it, i), st = blk & 1;
-          if (opens(i)) {
-            if (!(ok = wait(BAR_V_FULL + st, blk >> 1))) break;
-            clear(C::OFF_KV + st * 2 * C::TILE_BYTES + C::TILE_BYTES, ((it.first + i) >> 1) * BKV);
+          const bool more = j + 1 < it.blocks;
+          if constexpr (C::OWN_P) {
+            ok = (!more || (issue_s(0, j + 1) && issue_s(1, j + 1))) && issue_pv(0, j) && issue_pv(1, j);
+          } else {
+            // S held P of this block: its P V was issued before and the tensor pipe runs in order
+            ok = issue_pv(0, j) && (!more || issue_s(0, j + 1)) && issue_pv(1, j) && (!more || issue_s(1, j + 1));
           }
-          if (i == 0 && full > 0 && !(ok = wait(BAR_O_FREE + t, full - 1))) break;
-          if (!(ok = wait(BAR_P_FULL + 2 * t + (g & 1), g >> 1))) break;
-          tc_fence_after();
-          const uint32_t vb = v_lo + st * STAGE16 + ((it.first + i) & 1) * HALF16;
-          const uint32_t d_tmem = tmem_base + C::COL_O + t * D;
-          const uint32_t p_tmem = tmem_base + C::COL_S + t * 128 + (g & 1) * SUB;  // P: keys 2k, 2k+1 in column k
-          if (elect_one()) {
-#pragma unroll
-            for (int kk = 0; kk < SUB / 16; ++kk) umma_bf16_tmem_a(d_tmem, p_tmem + kk * 8, vb + ((kk * 2048) >> 4), HI, idesc_o, (i | kk) != 0);
-            umma_commit(bar(BAR_O_DONE + t));
-            if (i == it.steps - 1) umma_commit(bar(BAR_O_LAST + t));
-            if (closes(i)) umma_commit(bar(BAR_V_EMPTY + st));
-          }
-          __syncwarp();
-          // S of the step after the next takes the place of this step's P, once P V has read it: nothing orders products with different
-          // accumulators.  The softmax works on the step between them meanwhile.
-          if (i + 2 < it.steps) ok = wait(BAR_O_DONE + t, g) && issue_s(i + 2);
         }
-        // the next item's first S take the places of the last two P
-        if (ok) ok = wait(BAR_O_DONE + t, steps + it.steps - 1);
-        steps += it.steps;
-        blocks += stage_of(it, it.steps - 1) + 1;
+        blocks += it.blocks;
         ++full;
       }
     } else if (warp == 2) {
@@ -360,7 +349,8 @@ attention_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
       const int n_rows = (p.seq + cta_rows - 1) / cta_rows, per_row = p.batch * cta_heads;
       int next = static_cast<int>(blockIdx.x);
       for (int k = 0;; ++k) {
-        Item it = {-1, 0, 0, 0, 0};
+        Item it = {};
+        it.batch = -1;
         if (next >= 0) {
           // late queries first: under a causal mask they see the most
           it.query = (n_rows - 1 - next / per_row) * cta_rows;
@@ -368,8 +358,13 @@ attention_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
           it.batch = bh / cta_heads;
           it.head = bh % cta_heads * (p.pair_heads ? TILES : 1);
           const ftb200::KeyRange r = p.mask.keys_of(it.batch, it.query, p.pair_heads ? 1 : TILES, p.seq);
-          it.first = r.lo / SUB;
-          it.steps = r.hi > r.lo ? (r.hi + SUB - 1) / SUB - it.first : 0;
+          it.first = r.lo;
+          it.blocks = r.hi > r.lo ? (r.hi - r.lo + BKV - 1) / BKV : 0;
+          for (int t = 0; t < TILES; ++t) {
+            const ftb200::KeyRange a = p.mask.keys_of_all(it.batch, it.query + t * q_step, p.seq);
+            it.all_lo[t] = a.lo;
+            it.all_hi[t] = a.hi;
+          }
         }
         if (!wait(BAR_ITEM_EMPTY + (k & 1), (k >> 1) ^ 1)) break;
         if (lane == 0) items[k & 1] = it;
@@ -382,6 +377,7 @@ attention_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
         __syncwarp();
         if (!wait(BAR_CLAIMED, k)) break;
         next = claimed(answer);
+        if (next >= n_rows * per_row) next = -1;
         fence_async_smem();  // read before the next answer is written
         __syncwarp();
       }
@@ -395,39 +391,49 @@ attention_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
     const int row = quarter * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_addr = tmem_base + C::COL_S + t * 128 + lane_addr;
+    const uint32_t p_addr = tmem_base + C::COL_P + t * C::P_STEP + lane_addr;
     const uint32_t o_addr = tmem_base + C::COL_O + t * D + lane_addr;
     const uint32_t off_stage = C::OFF_O + (warp - 4) * 4096;
     uint8_t* stage = smem + off_stage + lane * 128;
     // with SCORE the scores come scaled, in units of log2
     const float scale_log2 = SCORE ? 1.f : p.scale_log2;
-    Item it;
-    ftb200::RowMask mine = {0, 0, 0, 0};
-    int steps = 0, full = 0;
-    bool ok = read_item(0, it);
-    if (ok && it.batch >= 0) mine = p.mask.row(it.batch, it.query + t * q_step + row, p.seq);
-    for (int k = 0; ok && it.batch >= 0; ++k) {
+    // The item stays in shared memory while the softmax works on it, and of the row's mask only the ends are kept: registers are scarce.
+    int blocks = 0, full = 0;
+    bool ok = true;
+    for (int k = 0;; ++k) {
+      if (!(ok = wait(BAR_ITEM_FULL + (k & 1), k >> 1))) break;
+      const Item& it = items[k & 1];
+      if (it.batch < 0) break;
       const int query = it.query + t * q_step + row;
       const int head = it.head + t * h_step;
+      const ftb200::KeyRange mine = p.mask.row(it.batch, query, p.seq);
       float slope2 = 0.f;
       if constexpr (SCORE) slope2 = p.mask.slope2(head);
       float m_used = -INFINITY, l_sum = 0.f;
-      for (int i = 0; i < it.steps; ++i) {
-        const int g = steps + i;
-        if (!(ok = wait(BAR_S_FULL + 2 * t + (g & 1), g >> 1))) break;
+      for (int j = 0; j < it.blocks; ++j) {
+        const int g = blocks + j;
+        if (!(ok = wait(BAR_S_FULL + t, g))) break;
         tc_fence_after();
-        const uint32_t at = s_addr + (g & 1) * SUB;
-        uint32_t sv[SUB];
-        tmem_ld32(at, sv);
-        tmem_ld32(at + 32, sv + 32);
-        tmem_wait_ld();
-        const int first = (it.first + i) * SUB;
-        if constexpr (SCORE) {
-          p.mask.cap_scores<SUB>(sv);
-          p.mask.slope_scores<SUB>(sv, static_cast<float>(query - first), -1.f, slope2);
-        }
-        if (!mine.all(first, SUB)) {
+        uint32_t sv[BKV];
 #pragma unroll
-          for (int w = 0; w < SUB / 32; ++w) {
+        for (int c = 0; c < BKV / 32; ++c) tmem_ld32(s_addr + c * 32, sv + c * 32);
+        tmem_wait_ld();
+        if constexpr (C::OWN_P) {
+          tc_fence_before();
+          mbar_arrive_warp(bar(BAR_S_READ + t));
+        }
+        const int first = it.first + j * BKV;
+        if constexpr (SCORE) {
+          p.mask.cap_scores<BKV>(sv);
+          if (p.mask.slopes != nullptr) {
+            const float far = static_cast<float>(query - first);
+#pragma unroll
+            for (int c = 0; c < BKV; ++c) sv[c] = __float_as_uint(fmaf(-slope2, fabsf(far - c), __uint_as_float(sv[c])));
+          }
+        }
+        if (first < it.all_lo[t] || first + BKV > it.all_hi[t]) {
+#pragma unroll
+          for (int w = 0; w < BKV / 32; ++w) {
             const uint32_t bits = ftb200::range_bits(mine.lo - first - 32 * w, mine.hi - first - 32 * w);
 #pragma unroll
             for (int c = 0; c < 32; ++c)
@@ -436,25 +442,27 @@ attention_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
         }
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < SUB; c += 2)
+        for (int c = 0; c < BKV; c += 2)
           mx4[(c >> 1) & 3] = fmaxf(fmaxf(mx4[(c >> 1) & 3], __uint_as_float(sv[c])), __uint_as_float(sv[c + 1]));
         const float m_new = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
 
         // raise the maximum only when it moved far
         float alpha = 1.f;
-        const bool raise = i > 0 && (m_new - m_used) * scale_log2 > RESCALE_THRESHOLD;
+        const bool raise = j > 0 && (m_new - m_used) * scale_log2 > RESCALE_THRESHOLD;
         const bool any_raise = __any_sync(0xffffffffu, raise);
-        if (i == 0) {
+        if (j == 0) {
           m_used = m_new;
         } else if (raise) {
           alpha = exp2f((m_used - m_new) * scale_log2);
           m_used = m_new;
           l_sum *= alpha;
         }
-        if (any_raise) {
-          // O may only be touched once P V of the previous step is done; P V of this step waits for P
+        // O, and P where it has columns of its own, may only be touched once P V of the previous block is done; P V of this block waits for P
+        if ((any_raise || C::OWN_P) && g > 0) {
           if (!(ok = wait(BAR_O_DONE + t, g - 1))) break;
           tc_fence_after();
+        }
+        if (any_raise) {
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
             uint32_t ov[32];
@@ -470,7 +478,7 @@ attention_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
         const unsigned long long scale2 = f2_pack(scale_log2, scale_log2), neg_m2 = f2_pack(neg_m, neg_m);
         unsigned long long sum2[2] = {0ull, 0ull};
 #pragma unroll
-        for (int c = 0; c < SUB / 32; ++c) {
+        for (int c = 0; c < BKV / 32; ++c) {
           uint32_t packed[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
@@ -491,27 +499,25 @@ attention_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
             __nv_bfloat162 pk = __floats2bfloat162_rn(p0, p1);
             packed[e] = *reinterpret_cast<uint32_t*>(&pk);
           }
-          // P replaces the first half of the scores this thread has already taken into registers
-          tmem_st16(at + c * 16, packed);
+          tmem_st16(p_addr + c * 16, packed);  // the scores are in registers
+          if (c == 1) {
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive_warp(bar(BAR_P_HALF + t));
+          }
         }
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive_warp(bar(BAR_P_FULL + 2 * t + (g & 1)));
+        mbar_arrive_warp(bar(BAR_P_FULL + t));
         float sum4[4];
         f2_unpack(sum2[0], sum4[0], sum4[1]);
         f2_unpack(sum2[1], sum4[2], sum4[3]);
         l_sum += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
       }
       if (!ok) break;
-      steps += it.steps;
+      blocks += it.blocks;
 
-      // the next item's rows are on their way while this one's leave
-      Item next;
-      if (!(ok = read_item(k + 1, next))) break;
-      ftb200::RowMask theirs = {0, 0, 0, 0};
-      if (next.batch >= 0) theirs = p.mask.row(next.batch, next.query + t * q_step + row, p.seq);
-
-      if (it.steps > 0) {
+      if (it.blocks > 0) {
         if (!(ok = wait(BAR_O_LAST + t, full))) break;
         ++full;
       }
@@ -526,7 +532,7 @@ attention_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
         tmem_ld32(o_addr + s * 64, ov);
         tmem_ld32(o_addr + s * 64 + 32, ov + 32);
         tmem_wait_ld();
-        if (s == C::SLABS - 1 && it.steps > 0) {
+        if (s == C::SLABS - 1 && it.blocks > 0) {
           tc_fence_before();
           mbar_arrive_warp(bar(BAR_O_FREE + t));
         }
@@ -555,8 +561,7 @@ attention_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
         p.lse[(static_cast<long long>(it.batch) * p.n_heads + head) * p.seq + query] =
             nothing ? -INFINITY : (m_used * scale_log2 + log2f(l_sum)) * 0.6931471805599453f;
       }
-      it = next;
-      mine = theirs;
+      mbar_arrive_warp(bar(BAR_ITEM_EMPTY + (k & 1)));
     }
     if (lane == 0) bulk_wait_read();
     __syncwarp();

@@ -33,7 +33,7 @@ struct KeyRange {
   int lo, hi;
 };
 
-// A query's keys [lo, hi), and the keys [all_lo, all_hi) that every query of its tile sees.
+// A key's queries [lo, hi), and the queries [all_lo, all_hi) that see every key of its tile.
 struct RowMask {
   int lo, hi, all_lo, all_hi;
   __device__ __forceinline__ bool all(int first, int n) const { return all_lo <= first && first + n <= all_hi; }
@@ -69,18 +69,20 @@ struct MaskParams {
     return r;
   }
 
-  __device__ __forceinline__ RowMask row(int b, int query, int seq) const {
-    RowMask m = {0, 0, INT_MAX, 0};
-    if (query >= seq) return m;
-    if (rows == nullptr) {
-      m.hi = causal ? query + 1 : seq;
-      m.all_lo = 0;
-      m.all_hi = causal ? query / 128 * 128 + 1 : seq;
-      return m;
-    }
-    const int4 r = rows[static_cast<long long>(b) * seq + query];
-    const int4 x = tile(b, query / 128, seq, 0);
-    return {r.x, r.y, x.z, x.w};
+  // Keys that each of the 128 queries from q0 on sees (of those inside the sequence).
+  __device__ __forceinline__ KeyRange keys_of_all(int b, int q0, int seq) const {
+    if (q0 >= seq) return {INT_MAX, 0};
+    if (rows == nullptr) return {0, causal ? q0 + 1 : seq};
+    const int4 x = tile(b, q0 / 128, seq, 0);
+    return {x.z, x.w};
+  }
+
+  // A query's keys.
+  __device__ __forceinline__ KeyRange row(int b, int query, int seq) const {
+    if (query >= seq) return {0, 0};
+    if (rows == nullptr) return {0, causal ? query + 1 : seq};
+    const int2 r = *reinterpret_cast<const int2*>(rows + static_cast<long long>(b) * seq + query);
+    return {r.x, r.y};
   }
 
   // The other way round: the queries that the block of 128 keys looks at, and those that see a key.
@@ -116,12 +118,12 @@ struct MaskParams {
     return __any_sync(0xffffffffu, any);
   }
 
-  // Rows of a tile in shared memory (slabs of 128 rows x 128 bytes) that belong to padding become zeros, by one warp: what stands in padding may
-  // be anything, and zero times infinity would reach the tile's other rows.  The products that follow see it.
-  __device__ __forceinline__ void clear_padding(uint8_t* tile_mem, int slabs, int b, int t, int seq, int lane) const {
-    if (tile(b, t, seq, 0).z != INT_MAX) return;
-    for (int r = lane; r < 128 && t * 128 + r < seq; r += 32) {
-      const int4 x = rows[static_cast<long long>(b) * seq + t * 128 + r];
+  // Of a tile in shared memory (slabs of 128 rows x 128 bytes; its first row is row `first` of the sequence) the rows that belong to padding
+  // become zeros, by one warp: what stands in padding may be anything, and zero times infinity would reach the tile's other rows.  The
+  // products that follow see it.
+  __device__ __forceinline__ void clear_padding(uint8_t* tile_mem, int slabs, int b, int first, int seq, int lane) const {
+    for (int r = lane; r < 128 && first + r < seq; r += 32) {
+      const int4 x = rows[static_cast<long long>(b) * seq + first + r];
       if (x.y > x.x) continue;
       for (int s = 0; s < slabs; ++s)
         for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(tile_mem + s * (128 * 128) + r * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
@@ -152,10 +154,9 @@ struct MaskParams {
     }
   }
 
-  // A thread's N products become log2(e) softcap tanh(scale s / softcap), or log2(e) scale s without a cap.
+  // N products of each thread of a warp become log2(e) softcap tanh(scale s / softcap), or log2(e) scale s without a cap.
   template <int N>
   __device__ __forceinline__ void cap_scores(uint32_t* sv) const {
-    using namespace tc;
     if (capped) {
       float big[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -168,23 +169,13 @@ struct MaskParams {
         by_polynomial<N, 6>(sv, poly);
       } else {
 #pragma unroll
-        for (int c = 0; c < N; ++c) {
-          const float e = exp2f(__uint_as_float(sv[c]) * in2);
-          sv[c] = __float_as_uint(fmaf(-2.f * cap2, __frcp_rn(e + 1.f), cap2));
-        }
+        for (int c = 0; c < N; ++c)
+          sv[c] = __float_as_uint(fmaf(-2.f * cap2, __frcp_rn(exp2f(__uint_as_float(sv[c]) * in2) + 1.f), cap2));
       }
     } else {
 #pragma unroll
       for (int c = 0; c < N; ++c) sv[c] = __float_as_uint(__uint_as_float(sv[c]) * scale_log2);
     }
-  }
-
-  // The slope's part, for score c at the distance |far + c step| (step 1 or -1).
-  template <int N>
-  __device__ __forceinline__ void slope_scores(uint32_t* sv, float far, float step, float slope2) const {
-    if (slopes == nullptr) return;
-#pragma unroll
-    for (int c = 0; c < N; ++c) sv[c] = __float_as_uint(fmaf(-slope2, fabsf(far + c * step), __uint_as_float(sv[c])));
   }
 };
 
