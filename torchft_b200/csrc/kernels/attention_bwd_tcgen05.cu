@@ -51,6 +51,7 @@
 #include <math.h>
 
 #include <initializer_list>
+#include <type_traits>
 
 #include "attention_masks.cuh"
 #include "ftb200_common.cuh"
@@ -477,34 +478,42 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         const float slope2 = p.mask.slope2(w.h);
         const float far = static_cast<float>(w.qt * BQ + g * CPT - (jb * BKV + row));
         const bool all = mine.all(w.qt * BQ, BQ);
+        const unsigned long long inv2 = f2_pack(p.mask.neg_inv_cap2_sq, p.mask.neg_inv_cap2_sq), one2 = f2_pack(1.f, 1.f);
+        auto probabilities = [&](auto partial) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int q0 = w.qt * BQ + g * CPT + half * 32;
-          const uint32_t bits = all ? 0xffffffffu : ftb200::range_bits(mine.lo - q0, mine.hi - q0);
-          uint32_t pt[16];
+          for (int half = 0; half < 2; ++half) {
+            const int q0 = w.qt * BQ + g * CPT + half * 32;
+            const uint32_t bits = decltype(partial)::value ? ftb200::range_bits(mine.lo - q0, mine.hi - q0) : 0u;
+            uint32_t pt[16];
 #pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            const int qi = half * 32 + 2 * c;
-            const ulonglong2 l4 = lse2[qi / 4];
-            float y0 = __uint_as_float(sv[qi]), y1 = __uint_as_float(sv[qi + 1]), x0, x1;
-            f2_unpack(f2_add(f2_pack(y0, y1), c % 2 == 0 ? l4.x : l4.y), x0, x1);
-            if (p.mask.slopes != nullptr) {
-              x0 = fmaf(-slope2, fabsf(far + qi), x0);
-              x1 = fmaf(-slope2, fabsf(far + (qi + 1)), x1);
+            for (int c = 0; c < 16; ++c) {
+              const int qi = half * 32 + 2 * c;
+              const ulonglong2 l4 = lse2[qi / 4];
+              const unsigned long long y = f2_pack(__uint_as_float(sv[qi]), __uint_as_float(sv[qi + 1]));
+              float x0, x1;
+              f2_unpack(f2_add(y, c % 2 == 0 ? l4.x : l4.y), x0, x1);
+              if (p.mask.slopes != nullptr) {
+                x0 = fmaf(-slope2, fabsf(far + qi), x0);
+                x1 = fmaf(-slope2, fabsf(far + (qi + 1)), x1);
+              }
+              x0 = exp2f(x0);
+              x1 = exp2f(x1);
+              if constexpr (decltype(partial)::value) {
+                x0 = bits >> (2 * c) & 1u ? x0 : 0.f;
+                x1 = bits >> (2 * c + 1) & 1u ? x1 : 0.f;
+              }
+              __nv_bfloat162 a = __floats2bfloat162_rn(x0, x1);
+              pt[c] = *reinterpret_cast<uint32_t*>(&a);
+              // without a cap the factor is one
+              f2_unpack(f2_mul(f2_pack(x0, x1), f2_fma(f2_mul(y, inv2), y, one2)), pe[qi], pe[qi + 1]);
             }
-            x0 = bits >> (2 * c) & 1u ? exp2f(x0) : 0.f;
-            x1 = bits >> (2 * c + 1) & 1u ? exp2f(x1) : 0.f;
-            __nv_bfloat162 a = __floats2bfloat162_rn(x0, x1);
-            pt[c] = *reinterpret_cast<uint32_t*>(&a);
-            if (p.mask.capped) {
-              x0 *= fmaf(y0 * p.mask.neg_inv_cap2_sq, y0, 1.f);
-              x1 *= fmaf(y1 * p.mask.neg_inv_cap2_sq, y1, 1.f);
-            }
-            pe[qi] = x0;
-            pe[qi + 1] = x1;
+            tmem_st16(s_addr + half * 16, pt);  // over scores that this thread has read
           }
-          tmem_st16(s_addr + half * 16, pt);  // over scores that this thread has read
-        }
+        };
+        if (all)
+          probabilities(std::false_type());
+        else
+          probabilities(std::true_type());
         tmem_wait_st();
       } else {
         uint32_t sv[CPT];
