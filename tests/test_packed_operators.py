@@ -275,8 +275,8 @@ def test_c_entries_refuse_before_they_launch():
     assert K._fn("layernorm_fwd")(a, None, None, a, None, a, a, a, 4, 12, 1e-5, 0, None) == -1
     assert K._fn("layernorm_fwd")(odd, None, None, a, None, a, a, a, 4, 16, 1e-5, 0, None) == -2
     assert K._fn("layernorm_fwd")(a, None, None, a, None, a, a, a, 4, 16392, 1e-5, 0, None) == -4
-    assert K._fn("layernorm_bwd")(a, a, a, a, a, None, a, a, None, a, 4, 16392, 0, 0, None) == -4
-    assert K._fn("layernorm_bwd")(a, odd, a, a, a, None, a, a, None, a, 4, 16, 0, 0, None) == -2
+    assert K._fn("layernorm_bwd")(a, a, a, a, a, None, a, a, None, a, 4, 16392, 0, 0, None, None) == -4
+    assert K._fn("layernorm_bwd")(a, odd, a, a, a, None, a, a, None, a, 4, 16, 0, 0, None, None) == -2
     assert K._fn("rope_axes")(odd, a, a, a, 4, 1, 2, 16, 32, 0, 0, 0, None) == -2
     assert K._fn("rope_axes")(a, a, a, a, 4, 1, 2, 20, 40, 0, 0, 0, None) == -2
     assert K._fn("rope_axes")(a, a, a, a, 4, 1, 2, 16, 36, 0, 0, 0, None) == -2

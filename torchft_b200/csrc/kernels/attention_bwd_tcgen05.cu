@@ -146,12 +146,6 @@ __device__ __forceinline__ void rotate_back(float* f, const float4& c0, const fl
   }
 }
 
-__device__ __forceinline__ void bulk_load_1d(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
-}
-
 // Adds `bytes` of shared memory to global memory as fp32.  The calling thread's bulk group has to be committed.
 __device__ __forceinline__ void bulk_add_f32(float* dst, uint32_t src, uint32_t bytes) {
   asm volatile("cp.reduce.async.bulk.global.shared::cta.bulk_group.add.f32 [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes)
@@ -276,8 +270,8 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 #pragma unroll
           for (int sl = 0; sl < SLABS; ++sl)
             tma_load_3d(sq + sl * SLAB, &tmQ, bar(BAR_Q_FULL + st), w.h * D + 64 * sl, q0, b);
-          bulk_load_1d(sst, p.neg_lse2 + stat_off, BQ * 4, bar(BAR_Q_FULL + st));
-          bulk_load_1d(sst + BQ * 4, p.neg_delta + stat_off, BQ * 4, bar(BAR_Q_FULL + st));
+          bulk_load(sst, p.neg_lse2 + stat_off, BQ * 4, bar(BAR_Q_FULL + st));
+          bulk_load(sst + BQ * 4, p.neg_delta + stat_off, BQ * 4, bar(BAR_Q_FULL + st));
         }
         __syncwarp();
         if (!mbar_wait_warp(bar(BAR_DO_EMPTY + dst), static_cast<uint32_t>(t / Ly::DO_STAGES) & 1u ^ 1u, abort_flag)) {

@@ -10,6 +10,7 @@
 #include <type_traits>
 
 #include "ftb200_common.cuh"
+#include "tcgen05_helpers.cuh"
 
 namespace {
 
@@ -143,39 +144,79 @@ layernorm_fwd_kernel(const typename Row<T>::V* x, const typename Row<T>::V* res,
 }
 
 constexpr int BWD_THREADS = 512;
+constexpr int MAX_STAGES = 8;
+constexpr int RING_BYTES = 196608;  // of shared memory, for rows on their way
 
 // A group keeps its columns over all its rows, so dw and db accumulate in registers; the groups of a block meet in shared memory at the
-// end and leave one row of partial sums each of dw and db.  One block per SM.
+// end and leave one row of partial sums each of dw and db.  One block per SM.  The rows that a group will work on next (dy, x, dres) are on their
+// way into a ring of its own, as many as there is room for (bulk copies; 2048 elements of bf16: 4 groups x 4 rows x 12 KB).  With a row's
+// loads in registers there was room for one: 8192 x 2048 34.7 us (29.9 now, both kernels, 4.5 TB/s), 8192 x 4096 65.7 (49.1, 5.5 TB/s).
 template <typename T, int TPR, int VPT>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
 layernorm_bwd_kernel(const typename Row<T>::V* dy, const typename Row<T>::V* x, const typename Row<T>::V* w, const float* mean, const float* rstd,
-                     const typename Row<T>::V* dres, typename Row<T>::V* dx, float* partial, long long rows, int D8) {
-  ftb200::wait_for_previous();
-  ftb200::start_next();
+                     const typename Row<T>::V* dres, typename Row<T>::V* dx, float* partial, long long rows, int D8, int stages, int* status) {
+  using namespace ftb200::tc;
   using V = typename Row<T>::V;
   constexpr int GROUPS = BWD_THREADS / TPR;
+  extern __shared__ __align__(128) uint8_t ring[];  // [group][stage][dy, x, dres][D8]
   __shared__ float part[2][BWD_THREADS / 32 * 2];
   __shared__ float4 meet[BWD_THREADS][2];
+  __shared__ uint64_t bars[GROUPS * MAX_STAGES];
+  __shared__ volatile int abort_flag;
   const int g = threadIdx.x / TPR, i0 = threadIdx.x % TPR;
+  const int n_in = dres != nullptr ? 3 : 2;
+  const uint32_t row_bytes = D8 * static_cast<uint32_t>(sizeof(V));
+  uint8_t* mine = ring + g * stages * n_in * row_bytes;
+  const uint32_t bar = smem_u32(bars + g * MAX_STAGES);
+  if (threadIdx.x < GROUPS * MAX_STAGES) mbar_init(smem_u32(bars + threadIdx.x), 1);
+  if (threadIdx.x == 0) abort_flag = 0;
+  fence_async_smem();
+  __syncthreads();
+  ftb200::wait_for_previous();
+  ftb200::start_next();
+  const long long first = blockIdx.x + static_cast<long long>(gridDim.x) * g, step = static_cast<long long>(gridDim.x) * GROUPS;
+  auto fetch = [&](long long row, int s) {  // by the group's first thread
+    const uint32_t to = smem_u32(mine + s * n_in * row_bytes);
+    mbar_expect_tx(bar + 8 * s, n_in * row_bytes);
+    bulk_load(to, dy + row * D8, row_bytes, bar + 8 * s);
+    bulk_load(to + row_bytes, x + row * D8, row_bytes, bar + 8 * s);
+    if (n_in == 3) bulk_load(to + 2 * row_bytes, dres + row * D8, row_bytes, bar + 8 * s);
+  };
+  if (i0 == 0)
+    for (int s = 0; s < stages && first + s * step < rows; ++s) fetch(first + s * step, s);
   float acc[2][VPT][8];  // dw, db
 #pragma unroll
   for (int v = 0; v < VPT; ++v)
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[0][v][e] = acc[1][v][e] = 0.f;
   const float inv_d = 1.f / (8.f * D8);
-  int turn = 0;
-  for (long long row = blockIdx.x + static_cast<long long>(gridDim.x) * g; row < rows; row += static_cast<long long>(gridDim.x) * GROUPS) {
+  V wv[VPT];
+  auto weights = [&] {
+#pragma unroll
+    for (int v = 0; v < VPT; ++v)
+      if (i0 + v * TPR < D8) wv[v] = w[i0 + v * TPR];
+  };
+  if constexpr (VPT <= 2) weights();
+  int turn = 0, s = 0;
+  uint32_t phase = 0;
+  float m = 0.f, r = 0.f;
+  if (first < rows) m = mean[first], r = rstd[first];
+  for (long long row = first; row < rows; row += step) {
+    mbar_wait(bar + 8 * s, phase, &abort_flag);  // should it run out, the group goes on together: the status word tells
     V a[VPT], b[VPT], d[VPT];
+    const V* from = reinterpret_cast<const V*>(mine + s * n_in * row_bytes);
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int i = i0 + v * TPR;
       if (i < D8) {
-        a[v] = dy[row * D8 + i];
-        b[v] = x[row * D8 + i];
-        if (dres != nullptr) d[v] = dres[row * D8 + i];
+        a[v] = from[i];
+        b[v] = from[D8 + i];
+        if (dres != nullptr) d[v] = from[2 * D8 + i];
       }
     }
-    const float m = mean[row], r = rstd[row];
+    float m_next = 0.f, r_next = 0.f;
+    if (row + step < rows) m_next = mean[row + step], r_next = rstd[row + step];
+    if constexpr (VPT > 2) weights();
     float sums[2] = {0.f, 0.f};  // of g and of g xh
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
@@ -183,7 +224,7 @@ layernorm_bwd_kernel(const typename Row<T>::V* dy, const typename Row<T>::V* x, 
         float fa[8], fb[8], c[8];
         unpack8(a[v], fa);
         unpack8(b[v], fb);
-        unpack8(w[i0 + v * TPR], c);
+        unpack8(wv[v], c);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float xh = (fb[e] - m) * r, t = fa[e] * c[e];
@@ -196,7 +237,15 @@ layernorm_bwd_kernel(const typename Row<T>::V* dy, const typename Row<T>::V* x, 
     }
     group_sums<TPR>(sums, part[turn]);
     turn ^= 1;
+    if constexpr (TPR == 32) __syncwarp();
+    // the group has read the stage
+    if (i0 == 0 && row + stages * step < rows) fetch(row + stages * step, s);
+    if (++s == stages) {
+      s = 0;
+      phase ^= 1u;
+    }
     const float c0 = sums[0] * inv_d, c1 = sums[1] * inv_d;
+    if constexpr (VPT > 2) weights();  // no registers to keep them in
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int i = i0 + v * TPR;
@@ -204,7 +253,7 @@ layernorm_bwd_kernel(const typename Row<T>::V* dy, const typename Row<T>::V* x, 
         float fa[8], fb[8], c[8], o[8];
         unpack8(a[v], fa);
         unpack8(b[v], fb);
-        unpack8(w[i], c);
+        unpack8(wv[v], c);
 #pragma unroll
         for (int e = 0; e < 8; ++e) o[e] = r * (fmaf(fa[e], c[e], -c0) - (fb[e] - m) * r * c1);
         if (dres != nullptr) {
@@ -216,6 +265,13 @@ layernorm_bwd_kernel(const typename Row<T>::V* dy, const typename Row<T>::V* x, 
         store8(o, &dx[row * D8 + i]);
       }
     }
+    m = m_next, r = r_next;
+  }
+  __syncthreads();
+  if (abort_flag) {
+    if (threadIdx.x == 0 && status != nullptr) atomicExch(status, FTB200_ST_TIMEOUT);
+    const uint64_t t0 = ftb200::globaltimer_ns();  // copies in flight land in this block's shared memory
+    while (ftb200::globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
   }
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
@@ -283,7 +339,8 @@ int fwd_shape(int D8, bool few, F&& f) {
   return FTB200_E_TOOBIG;
 }
 
-// Backward: at most 2 vectors a thread up to 8192 elements, for whose three rows and two sums there are registers.
+// Backward: at most 2 vectors a thread up to 8192 elements, for whose two sums there are registers.  (With 4 vectors and half the
+// threads 8192 x 2048 in bf16 takes 50 us instead of 30, with one and twice the threads 35.)
 template <typename F>
 int bwd_shape(int D8, F&& f) {
   auto is = [&](auto tpr, auto vpt) { return f(tpr, vpt); };
@@ -317,14 +374,22 @@ int bwd_blocks(long long rows) { return static_cast<int>(std::min<long long>((ro
 
 template <typename T>
 int layernorm_bwd(const void* dy, const void* x, const void* w, const float* mean, const float* rstd, const void* dres, void* dx, void* dw, void* db,
-                  float* partial, long long rows, int D, int accumulate, cudaStream_t stream) {
+                  float* partial, long long rows, int D, int accumulate, int* status, cudaStream_t stream) {
   using V = typename Row<T>::V;
   const int D8 = D / 8;
   return bwd_shape(D8, [&](auto tpr, auto vpt) -> int {
     constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
     const int blocks = bwd_blocks(rows);
-    ftb200::launch_after(layernorm_bwd_kernel<T, TPR, VPT>, blocks, BWD_THREADS, 0, stream, (const V*)dy, (const V*)x, (const V*)w, mean, rstd,
-                         (const V*)dres, (V*)dx, partial, rows, D8);
+    const int row_bytes = (dres == nullptr ? 2 : 3) * D * static_cast<int>(sizeof(T)) * (BWD_THREADS / TPR);
+    const int stages = std::max(1, std::min(MAX_STAGES, RING_BYTES / row_bytes));
+    static std::atomic<unsigned long long> ready{0};  // per device
+    if (!ftb200::once_per_device(ready)) {
+      if (cudaFuncSetAttribute(layernorm_bwd_kernel<T, TPR, VPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_BYTES) != cudaSuccess)
+        return FTB200_E_CUDA;
+      ftb200::done_on_device(ready);
+    }
+    ftb200::launch_after(layernorm_bwd_kernel<T, TPR, VPT>, blocks, BWD_THREADS, stages * row_bytes, stream, (const V*)dy, (const V*)x,
+                         (const V*)w, mean, rstd, (const V*)dres, (V*)dx, partial, rows, D8, stages, status);
     ftb200::launch_after(layernorm_columns_kernel<T>, (D + 31) / 32 * (db == nullptr ? 1 : 2), 1024, 0, stream, (const float*)partial, (T*)dw,
                          (T*)db, blocks, D, accumulate);
     return cudaGetLastError() == cudaSuccess ? 0 : FTB200_E_CUDA;
@@ -350,10 +415,11 @@ FTB200_API long long ftb200_layernorm_bwd_scratch_floats(int D) { return 2LL * f
 
 // dy, x (the h of the forward pass), dres (may be null), dx: [rows, D]; w, dw, db (may be null): [D].  dx may be dy, x or dres.
 FTB200_API int ftb200_layernorm_bwd(const void* dy, const void* x, const void* w, const float* mean, const float* rstd, const void* dres, void* dx,
-                                    void* dw, void* db, float* partial, long long rows, int D, int accumulate, int f32, cudaStream_t stream) {
+                                    void* dw, void* db, float* partial, long long rows, int D, int accumulate, int f32, int* status,
+                                    cudaStream_t stream) {
   if (rows <= 0 || D <= 0 || D % 8 != 0) return FTB200_E_BADARG;
   for (const void* p : {dy, x, w, dres, (const void*)dx, (const void*)partial})
     if (misaligned(p)) return FTB200_E_ALIGN;
-  return f32 ? layernorm_bwd<float>(dy, x, w, mean, rstd, dres, dx, dw, db, partial, rows, D, accumulate, stream)
-             : layernorm_bwd<__nv_bfloat16>(dy, x, w, mean, rstd, dres, dx, dw, db, partial, rows, D, accumulate, stream);
+  return f32 ? layernorm_bwd<float>(dy, x, w, mean, rstd, dres, dx, dw, db, partial, rows, D, accumulate, status, stream)
+             : layernorm_bwd<__nv_bfloat16>(dy, x, w, mean, rstd, dres, dx, dw, db, partial, rows, D, accumulate, status, stream);
 }

@@ -59,7 +59,7 @@ _ARGS = {
     "attention_bwd": "ppppppppppiiiiillllllllfippp", "gemm_bf16": "pppiiiiilllipip",
     "attention_spans": "ppppppiiiip", "attention_masked_fwd": "pppppppppiiiiillllffipp",
     "attention_masked_bwd": "ppppppppppppppiiiiillllllllffippp", "rope_axes": "ppppliiiliiip",
-    "layernorm_fwd": "pppppppplifip", "layernorm_bwd": "ppppppppppliiip",
+    "layernorm_fwd": "pppppppplifip", "layernorm_bwd": "ppppppppppliiipp",
 }
 _ARGS["gemm_bf16_2cta"] = _ARGS["gemm_bf16"]
 _KIND = {"p": c_void_p, "i": c_int, "l": c_ll, "f": c_float}
@@ -536,7 +536,7 @@ def layernorm_bwd(
           or scratch.data_ptr() % 16):
         raise ValueError(f"scratch must be {need} contiguous fp32 on {x.device}")
     N.check(_fn("layernorm_bwd")(_at(dy), _at(x), _at(w), _at(mean), _at(rstd), _at(dres), _at(dx), _at(dw), _at(db), _at(scratch), T, D,
-                                 int(accumulate), int(x.dtype == torch.float32), _stream()), "layernorm_bwd", launches=2)
+                                 int(accumulate), int(x.dtype == torch.float32), _status_ptr(x.device), _stream()), "layernorm_bwd", launches=2)
     return dx, dw, db
 
 
