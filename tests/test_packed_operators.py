@@ -1,4 +1,4 @@
-"""Attention under masks and changed scores, rotary positions with several axes and layer norm without a GPU: the plain forms against their
+"""Attention under masks and changed scores, rotary positions with several axes and layer norm: the plain forms against their
 definitions, gradients against differences, and what the entry points refuse."""
 import math
 
@@ -6,6 +6,9 @@ import pytest
 import torch
 
 from torchft_b200.ops import kernels as K
+
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 
 
 def _ids(*runs):
@@ -184,13 +187,14 @@ def test_layernorm_of_no_rows():
 # ------------------------------------------------------------------ refusals
 
 
-def test_refusals_of_spans():
-    ids = torch.zeros(2, 5, dtype=torch.int32)
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals_of_spans(device):
+    ids = torch.zeros(2, 5, dtype=torch.int32, device=device)
     for bad in (ids.long(), ids[0], ids.t()):
         with pytest.raises(ValueError):
             K.attention_spans(bad)
     with pytest.raises(ValueError):
-        K.attention_spans(ids, prefix=torch.zeros(2, 4, dtype=torch.bool))
+        K.attention_spans(ids, prefix=torch.zeros(2, 4, dtype=torch.bool, device=device))
     with pytest.raises(ValueError):
         K.attention_spans(ids, prefix=ids)
     for window in (-1, 2**31):
@@ -202,11 +206,12 @@ def test_refusals_of_spans():
         K.attention_spans(ids, causal=False, prefix=ids.bool())
 
 
-def test_refusals_of_masked_attention():
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals_of_masked_attention(device):
     B, S, H, G, D = 2, 8, 4, 2, 64
-    q, kv = torch.zeros(B * S, H * D, dtype=torch.bfloat16), torch.zeros(B * S, G * D, dtype=torch.bfloat16)
-    lse = torch.zeros(B, H, S)
-    spans = K.attention_spans(torch.zeros(B, S, dtype=torch.int32))
+    q, kv = torch.zeros(B * S, H * D, dtype=torch.bfloat16, device=device), torch.zeros(B * S, G * D, dtype=torch.bfloat16, device=device)
+    lse = torch.zeros(B, H, S, device=device)
+    spans = K.attention_spans(torch.zeros(B, S, dtype=torch.int32, device=device))
 
     def both(q=q, k=kv, lse=lse, heads=(H, G, D), spans=spans, dk=kv, **how):
         with pytest.raises(ValueError):
@@ -221,19 +226,20 @@ def test_refusals_of_masked_attention():
     both(lse=lse[:, :-1])
     both(heads=(H, 3, D))
     both(heads=(2 * H, 2 * G, 32))
-    both(spans=K.attention_spans(torch.zeros(B, S + 1, dtype=torch.int32)))
+    both(spans=K.attention_spans(torch.zeros(B, S + 1, dtype=torch.int32, device=device)))
     for cap in (-1.0, math.inf, math.nan):
         both(softcap=cap)
-    both(slopes=torch.zeros(H - 1))
-    both(slopes=torch.zeros(H).double())
+    both(slopes=torch.zeros(H - 1, device=device))
+    both(slopes=torch.zeros(H, device=device).double())
     with pytest.raises(ValueError):
         K.attention_bwd(q, kv, kv, q, q, lse, q, kv[:-1], kv, B, S, H, G, D, spans=spans)
 
 
-def test_refusals_of_rope_axes():
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals_of_rope_axes(device):
     T, n, D = 4, 2, 16
-    buf, pos = torch.zeros(T, 3 * D), torch.zeros(2, T, dtype=torch.int32)
-    inv, axis = K.rope_axes_freqs([4, 4], 10.0, "cpu")
+    buf, pos = torch.zeros(T, 3 * D, device=device), torch.zeros(2, T, dtype=torch.int32, device=device)
+    inv, axis = K.rope_axes_freqs([4, 4], 10.0, device)
     for args in ((buf.double(), pos, inv, axis, n, D), (buf.t(), pos, inv, axis, n, D), (buf, pos.long(), inv, axis, n, D),
                  (buf, pos[:, :-1], inv, axis, n, D), (buf, pos[0], inv, axis, n, D), (buf, pos, inv.float(), axis, n, D),
                  (buf, pos, inv[1:], axis, n, D), (buf, pos, inv, axis.long(), n, D), (buf, pos, inv, axis, 4, D), (buf, pos, inv, axis, 0, D),
@@ -242,8 +248,9 @@ def test_refusals_of_rope_axes():
             K.rope_axes_(*args)
 
 
-def test_refusals_of_layernorm():
-    x, w, s = torch.zeros(4, 16), torch.zeros(16), torch.zeros(4)
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals_of_layernorm(device):
+    x, w, s = torch.zeros(4, 16, device=device), torch.zeros(16, device=device), torch.zeros(4, device=device)
     for args in ((x.double(), w), (x[:, :12], w[:12]), (x[0], w), (x, w[1:]), (x, w.bfloat16()), (x, w, w[1:]), (x.t(), w)):
         with pytest.raises(ValueError):
             K.layernorm_fwd(*args)
@@ -260,12 +267,13 @@ def test_refusals_of_layernorm():
         K.layernorm_bwd(x, x, w, s, s, dw=w, accumulate=True)
 
 
-def test_tensors_on_two_devices_are_refused():
-    x, w = torch.zeros(4, 16), torch.zeros(16)
+@pytest.mark.parametrize("device", DEVICES)
+def test_tensors_on_two_devices_are_refused(device):
+    x, w = torch.zeros(4, 16, device=device), torch.zeros(16, device=device)
     with pytest.raises(ValueError):
         K.layernorm_fwd(x, w.to("meta"))
     with pytest.raises(ValueError):
-        K.attention_spans(torch.zeros(2, 5, dtype=torch.int32), prefix=torch.zeros(2, 5, dtype=torch.bool, device="meta"))
+        K.attention_spans(torch.zeros(2, 5, dtype=torch.int32, device=device), prefix=torch.zeros(2, 5, dtype=torch.bool, device="meta"))
 
 
 def test_c_entries_refuse_before_they_launch():
@@ -293,3 +301,18 @@ def test_c_entries_refuse_before_they_launch():
     assert bwd(32, a, a, 0.0) == -1 and bwd(64, odd, a, 0.0) == -2
     assert bwd(64, a, None, 0.0) == -1 and bwd(64, a, odd, 0.0) == -2 and bwd(64, a, a, -1.0) == -1 and bwd(64, a, a, math.nan) == -1
     assert lib is K.N.lib()
+
+
+def test_the_host_module_refuses_tensors_off_the_gpu():
+    host = K.N.host()
+    x, w, ids = torch.zeros(4, 16), torch.zeros(16), torch.zeros(1, 4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="on a GPU"):
+        host.layernorm_fwd(x, w, None, 1e-5, None, None, None, None, None)
+    with pytest.raises(ValueError, match="on a GPU"):
+        host.attention_spans(ids, None, True, 0)
+    with pytest.raises(TypeError):
+        host.attention_spans(ids, None, True)
+    with pytest.raises(TypeError):
+        host.attention_spans(None, None, True, 0)
+    with pytest.raises(TypeError):
+        host.attention_spans(ids, 3, True, 0)

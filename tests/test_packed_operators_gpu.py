@@ -3,6 +3,7 @@
 Bounds count roundings: u = 2^-8 is half a step of bf16.  P is rounded before P V, the output once more; dS before dS K and dS^T Q, and its
 delta is that of the rounded output.  What the fp32 sums and the exponentials add is below a twentieth of that (2e-4 of a probability where
 the products of a score add up to 50), hence the factor."""
+import concurrent.futures
 import math
 
 import pytest
@@ -466,3 +467,40 @@ def test_captured_and_replayed_on_two_streams():
             assert torch.equal(got[k], ref[k]), k
         # dQ is summed by atomics: fp32 sums in another order move a rounding by a step now and then
         assert ((got["dx"].double() - ref["dx"].double()).norm() / ref["dx"].double().norm()) < U
+
+
+def test_a_misaligned_tensor_is_refused():
+    T, D = 4, 64
+    at = lambda n, dtype: torch.zeros(n + 1, dtype=dtype, device="cuda")[1:]  # noqa: E731
+    x, odd, w = torch.zeros(T, D, device="cuda"), at(T * D, torch.float32).view(T, D), torch.ones(D, device="cuda")
+    _, mean, rstd, _ = K.layernorm_fwd(x, w)
+    for args in ((odd, w), (x, at(D, torch.float32))):
+        with pytest.raises(K.N.KernelError):
+            K.layernorm_fwd(*args)
+    with pytest.raises(K.N.KernelError):
+        K.layernorm_bwd(odd, x, w, mean, rstd)
+    q, spans = at(T * D, torch.bfloat16).view(T, D), K.attention_spans(torch.zeros(1, T, dtype=torch.int32, device="cuda"))
+    with pytest.raises(K.N.KernelError):
+        K.attention_fwd(q, q, q, 1, T, 1, 1, D, torch.empty_like(q), spans=spans)
+
+
+def test_threads_with_streams_of_their_own():
+    B, S, H, G, D = 2, 300, 4, 2, 64
+    ids, _ = _documents(B, S, 40)
+    qkv, do = _packed(B, S, H, G, D, 3)
+    spans = K.attention_spans(ids)
+    want = _run_no_check(qkv, do, B, S, H, G, D, spans=spans)
+    torch.cuda.synchronize()
+
+    def work(_):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = [_run_no_check(qkv, do, B, S, H, G, D, spans=K.attention_spans(ids)) for _ in range(20)]
+            torch.cuda.current_stream().synchronize()
+        return got
+
+    with concurrent.futures.ThreadPoolExecutor(4) as pool:
+        for many in pool.map(work, range(4)):
+            for got in many:
+                assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+                # dQ is summed by atomics, as above
+                assert (got[2].double() - want[2].double()).norm() / want[2].double().norm() < U

@@ -1,10 +1,12 @@
 """In-tree native build for torchft_b200.
 
-Two shared objects are produced next to the Python sources so that they travel
+Three shared objects are produced next to the Python sources so that they travel
 with the source tree:
 
 * ``torchft_b200/_lib/libftb200_kernels.so`` -- every hand-written sm_100a CUDA
   kernel, exported through a plain C ABI (loaded with ``ctypes``).
+* ``torchft_b200/_ops_host.<ext-suffix>.so`` -- argument checks, result tensors and calls
+  of some operators in one C++ call each (a CPython module against torch's headers).
 * ``torchft_b200/_ftcp.<ext-suffix>.so``   -- the C++ control plane (lighthouse,
   manager server/client, quorum math) as a pybind11 module.
 
@@ -17,6 +19,7 @@ for ``sm_100a`` on machines without a GPU.
 from __future__ import annotations
 
 import hashlib
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -36,6 +39,7 @@ BUILD_DIR = REPO_DIR / "build"
 KERNEL_LIB = LIB_DIR / "libftb200_kernels.so"
 KERNEL_LIB_CHECKED = LIB_DIR / "libftb200_kernels_checked.so"  # -DFT_BOUNDS_CHECK=1 debug build
 CONTROL_MOD = PKG_DIR / ("_ftcp" + sysconfig.get_config_var("EXT_SUFFIX"))
+HOST_MOD = PKG_DIR / ("_ops_host" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 NVCC_FLAGS = [
     "-gencode",
@@ -175,10 +179,34 @@ def build_control() -> Path:
         return CONTROL_MOD
 
 
+def build_host() -> Path:
+    """Compile the host side of the operators that have one in C++.  torch's libraries are found where ``import torch``
+    has loaded them, so the module carries no path of theirs."""
+    with _lock:
+        spec = importlib.util.find_spec("torch")  # found, not imported
+        if spec is None or not spec.submodule_search_locations:
+            raise RuntimeError("torch not found; cannot build torchft_b200's host module")
+        torch_dir = Path(spec.submodule_search_locations[0])
+        sources = sorted((CSRC / "host").glob("*.cpp"))
+        flags = [
+            "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall",
+            f"-I{sysconfig.get_paths()['include']}",
+            f"-I{torch_dir / 'include'}",
+            f"-I{torch_dir / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
+            f"-I{_cuda_home()}/include",
+        ]
+        objs = _compile_objects(sources, [torch_dir / "version.py"], ["g++"], flags, "h")  # another torch: compiled again
+        if _needs_link(HOST_MOD, objs):
+            libs = ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+            _run(["g++", "-shared", "-o", str(HOST_MOD), *map(str, objs), f"-L{torch_dir / 'lib'}", *libs])
+        return HOST_MOD
+
+
 def build_all(verbose: bool = False) -> None:
     build_kernels(verbose=verbose)
     build_kernels(checked=True)  # the checked-index debug variant, used by tests/test_bounds_check_build.py
     build_control()
+    build_host()
 
 
 if __name__ == "__main__":

@@ -8,6 +8,7 @@ that no GPU code path silently falls back to eager PyTorch.
 from __future__ import annotations
 
 import ctypes
+import importlib
 import os
 import threading
 from typing import Optional
@@ -80,6 +81,36 @@ def bounds_status() -> tuple:
         if st and not code:
             code, index = st, int(idx.value)
     return code, index
+
+
+_host = None
+# the entries that the host module calls, in its order
+_HOST_ENTRIES = ("attention_spans", "attention_masked_fwd", "attention_masked_bwd", "attention_bwd_scratch_bytes", "rope_axes", "layernorm_fwd",
+                 "layernorm_bwd", "layernorm_bwd_scratch_floats")
+
+
+def host():
+    """The C++ host side of some operators (``torchft_b200/_ops_host``), bound to the library of :func:`lib`.  Like that
+    it is mandatory where those operators run on a GPU."""
+    global _host
+    if _host is not None:
+        return _host
+    library = lib()
+    with _lock:
+        if _host is None:
+            if not _build.HOST_MOD.exists():
+                if os.environ.get("FTB200_NO_AUTOBUILD"):
+                    raise KernelError(f"{_build.HOST_MOD} is missing; run `python -m torchft_b200._build`")
+                _build.build_host()
+            module = importlib.import_module("torchft_b200._ops_host")
+            module.bind(check_host, *(ctypes.cast(getattr(library, "ftb200_" + e), c_void_p).value for e in _HOST_ENTRIES))
+            _host = module
+        return _host
+
+
+def check_host(rc: int, what: str) -> None:
+    """Raises for an error code that an entry gave to the host module."""
+    raise KernelError(f"{what}: {ERRORS.get(rc, rc)}")
 
 
 launch_count = 0  # kernels launched through this library since import (bench.py reports the delta)

@@ -387,12 +387,6 @@ def rmsnorm_bwd(
 # --------------------------------------------------------------------------- layer norm
 
 
-def _check_here(first: torch.Tensor) -> None:
-    """The tensors' device (``first`` is one of them) is the current one, on whose stream the kernel is launched."""
-    if first.is_cuda and first.get_device() != torch._C._cuda_getDevice():
-        raise ValueError(f"the tensors are on {first.device}, which is not the current device")
-
-
 def _check_like(names: str, dtype: torch.dtype, shape, device: int, *tensors: Optional[torch.Tensor]) -> None:
     """Each of ``tensors`` that is not None is contiguous, of the type and shape, and on the device (-1: the CPU)."""
     for i, t in enumerate(tensors):
@@ -432,6 +426,10 @@ def layernorm_fwd(
     """Returns ``(normed, mean, rstd, h)`` where ``h = x + res`` (or ``x``), rounded to the type of ``x``, and ``normed = (h - mean) *
     rstd * w (+ b)``.  Rows of up to 16384 elements, all tensors in bf16 or all in fp32 (``mean`` and ``rstd`` in fp32).  ``out`` and
     ``h_out`` may be ``x`` or ``res``."""
+    if x.is_cuda:
+        results = N.host().layernorm_fwd(x, w, b, eps, res, h_out, out, mean, rstd)
+        N.launch_count += x.shape[0] > 0
+        return results
     _check_norm(x)
     T, D = x.shape
     if mean is None:
@@ -442,24 +440,18 @@ def layernorm_fwd(
         h_out = torch.empty_like(x)
     if out is None:
         out = torch.empty_like(x)
-    _check_here(x)
     dtype, at = x.dtype, x.get_device()
     _check_like("x res h_out out", dtype, x.shape, at, x, res, h_out, out)
     _check_like("w b", dtype, (D,), at, w, b)
     _check_like("mean rstd", torch.float32, (T,), at, mean, rstd)
     if out is h_out and res is not None:
         raise ValueError("out and h_out are two results")
-    if T > 0:
-        if not x.is_cuda:
-            o, m, r, h = ref_layernorm_fwd(x, w, b, eps, res)
-            out.copy_(o)
-            mean.copy_(m)
-            rstd.copy_(r)
-            if res is not None:
-                h_out.copy_(h)
-        else:
-            N.check(_fn("layernorm_fwd")(_at(x), _at(res), _at(h_out) if res is not None else None, _at(w), _at(b), _at(out), _at(mean),
-                                         _at(rstd), T, D, eps, int(x.dtype == torch.float32), _stream()), "layernorm_fwd")
+    o, m, r, h = ref_layernorm_fwd(x, w, b, eps, res)
+    out.copy_(o)
+    mean.copy_(m)
+    rstd.copy_(r)
+    if res is not None:
+        h_out.copy_(h)
     return out, mean, rstd, h_out if res is not None else x
 
 
@@ -499,6 +491,10 @@ def layernorm_bwd(
     which may be ``dy``, ``x`` or ``dres``; with ``accumulate`` the sums are added to what ``dw`` and ``db`` hold.  The partial sums lie in
     ``scratch`` (fp32 on the device, :func:`layernorm_bwd_scratch_floats` of them or more) between the two kernels, by default in memory
     of this call's own."""
+    if x.is_cuda:
+        results = N.host().layernorm_bwd(dy, x, w, mean, rstd, dres, dx, dw, db, bias, accumulate, scratch, _status_ptr(x.device))
+        N.launch_count += 2 * (x.shape[0] > 0)
+        return results
     _check_norm(x)
     T, D = x.shape
     if accumulate and (dw is None or (bias and db is None)):
@@ -511,7 +507,6 @@ def layernorm_bwd(
         db = None
     elif db is None:
         db = torch.empty_like(w)
-    _check_here(x)
     dtype, at = x.dtype, x.get_device()
     _check_like("x dy dres dx", dtype, x.shape, at, x, dy, dres, dx)
     _check_like("w dw db", dtype, (D,), at, w, dw, db)
@@ -522,21 +517,11 @@ def layernorm_bwd(
             if db is not None:
                 db.zero_()
         return dx, dw, db
-    if not x.is_cuda:
-        rdx, rdw, rdb = ref_layernorm_bwd(dy, x, w, mean, rstd, dres)
-        dx.copy_(rdx)
-        dw.copy_(((dw.float() if accumulate else 0) + rdw).to(dw.dtype))
-        if db is not None:
-            db.copy_(((db.float() if accumulate else 0) + rdb).to(db.dtype))
-        return dx, dw, db
-    need = layernorm_bwd_scratch_floats(D)
-    if scratch is None:
-        scratch = torch.empty(need, dtype=torch.float32, device=x.device)
-    elif (scratch.device != x.device or scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < need
-          or scratch.data_ptr() % 16):
-        raise ValueError(f"scratch must be {need} contiguous fp32 on {x.device}")
-    N.check(_fn("layernorm_bwd")(_at(dy), _at(x), _at(w), _at(mean), _at(rstd), _at(dres), _at(dx), _at(dw), _at(db), _at(scratch), T, D,
-                                 int(accumulate), int(x.dtype == torch.float32), _status_ptr(x.device), _stream()), "layernorm_bwd", launches=2)
+    rdx, rdw, rdb = ref_layernorm_bwd(dy, x, w, mean, rstd, dres)
+    dx.copy_(rdx)
+    dw.copy_(((dw.float() if accumulate else 0) + rdw).to(dw.dtype))
+    if db is not None:
+        db.copy_(((db.float() if accumulate else 0) + rdb).to(db.dtype))
     return dx, dw, db
 
 
@@ -618,6 +603,9 @@ def rope_axes_(buf: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tenso
     ``inv_freq`` fp64 and ``axis`` int32, both ``[head_dim/2]``, see :func:`rope_axes_freqs`); an ``axis`` outside ``[0, axes)`` leaves the
     pair as it is.  Pairs are neighbours, as in :func:`rope_`, or with ``half`` elements ``j`` and ``j + head_dim/2``.  ``backward``
     turns back."""
+    if buf.is_cuda:
+        N.launch_count += N.host().rope_axes(buf, positions, inv_freq, axis, n_heads, head_dim, half, backward)
+        return buf
     if buf.dim() != 2 or buf.dtype not in (torch.bfloat16, torch.float32) or (buf.shape[1] > 1 and buf.stride(1) != 1):
         raise ValueError("buf must be a 2-D bf16 or fp32 tensor with unit inner stride")
     T = buf.shape[0]
@@ -626,18 +614,12 @@ def rope_axes_(buf: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tenso
         raise ValueError(f"buf of shape {tuple(buf.shape)} does not hold {n_heads} heads of {head_dim}")
     if positions.dim() != 2 or positions.shape[0] < 1:
         raise ValueError("positions must be contiguous int32 [axes, rows]")
-    _check_here(buf)
     at = buf.get_device()
     _check_like("positions", torch.int32, (positions.shape[0], T), at, positions)
     _check_like("inv_freq", torch.float64, (head_dim // 2,), at, inv_freq)
     _check_like("axis", torch.int32, (head_dim // 2,), at, axis)
-    if T == 0:
-        return buf
-    if not buf.is_cuda:
+    if T > 0:
         buf.copy_(ref_rope_axes(buf, positions, inv_freq, axis, n_heads, head_dim, half, backward))
-        return buf
-    N.check(_fn("rope_axes")(_at(buf), _at(positions), _at(inv_freq), _at(axis), T, positions.shape[0], n_heads, head_dim, ld,
-                             int(buf.dtype == torch.float32), int(half), int(backward), _stream()), "rope_axes")
     return buf
 
 
@@ -881,20 +863,17 @@ class AttentionSpans:
     ``positions`` int32 ``[batch, seq]`` counts from 0 in every document (``positions.view(1, -1)`` goes into :func:`rope_axes_`).
     ``tiles`` and ``padded`` are what the kernels need of 128 and of 1024 tokens."""
 
-    def __init__(self, batch: int, seq: int, device) -> None:
+    def __init__(self, batch: int, seq: int, device, buf: Optional[torch.Tensor] = None) -> None:
         self.batch, self.seq, self.n_tiles = batch, seq, (seq + 127) // 128
         a = 4 * batch * seq
         b = a + 8 * batch * self.n_tiles
         c = b + batch * seq
         self._at = (0, a, b, c, c + batch * ((seq + 1023) // 1024))
-        self._buf = torch.empty(self._at[4], dtype=torch.int32, device=device)
+        self._buf = torch.empty(self._at[4], dtype=torch.int32, device=device) if buf is None else buf
 
     @property
     def device(self) -> torch.device:
         return self._buf.device
-
-    def get_device(self) -> int:
-        return self._buf.get_device()
 
     def _part(self, i: int, *shape: int) -> torch.Tensor:
         return self._buf[self._at[i] : self._at[i + 1]].view(*shape)
@@ -914,11 +893,6 @@ class AttentionSpans:
     @property
     def padded(self) -> torch.Tensor:
         return self._part(3, self.batch, (self.seq + 1023) // 1024)
-
-    def _pointers(self) -> Tuple[int, int, int, int]:
-        base = self._buf.data_ptr()
-        _, a, b, c, _ = self._at
-        return base, base + 4 * a, base + 4 * b, base + 4 * c
 
 
 _NONE = 2**31 - 1
@@ -968,6 +942,10 @@ def attention_spans(documents: torch.Tensor, prefix: Optional[torch.Tensor] = No
     ``causal`` a token sees itself and those before it, at most the last ``window`` of them (itself among them) where that is not 0, and
     the tokens that ``prefix`` (bool or uint8 ``[batch, seq]``) flags at the start of a document are seen by all of it, by each other in
     both directions too."""
+    if documents.is_cuda:
+        buf = N.host().attention_spans(documents, prefix, causal, window)
+        N.launch_count += documents.numel() > 0
+        return AttentionSpans(*documents.shape, None, buf)
     if documents.dim() != 2 or documents.dtype != torch.int32 or not documents.is_contiguous():
         raise ValueError("documents must be contiguous int32 [batch, seq]")
     if prefix is not None:
@@ -978,18 +956,11 @@ def attention_spans(documents: torch.Tensor, prefix: Optional[torch.Tensor] = No
         raise ValueError("window must be 0 or a number of keys")
     if not causal and (window or prefix is not None):
         raise ValueError("a window or a prefix goes with a causal mask")
-    _check_here(documents)
     B, S = documents.shape
     spans = AttentionSpans(B, S, documents.device)
-    if B == 0 or S == 0:
-        return spans
-    if not documents.is_cuda:
+    if B > 0 and S > 0:
         for mine, t in zip((spans.rows, spans.positions, spans.tiles, spans.padded), ref_attention_spans(documents, prefix, causal, window)):
             mine.copy_(t)
-        return spans
-    rows, tiles, positions, padded = spans._pointers()
-    N.check(_fn("attention_spans")(_at(documents), _at(prefix), rows, positions, tiles, padded, B, S, int(causal), window, _stream()),
-            "attention_spans")
     return spans
 
 
@@ -1033,13 +1004,12 @@ def _check_masked(of_q, of_kv, spans: Optional[AttentionSpans], softcap: float, 
         raise ValueError("softcap must be 0 or a finite cap")
     if spans is not None and (spans.batch, spans.seq) != (batch, seq_len):
         raise ValueError(f"spans are of {(spans.batch, spans.seq)}, not of {(batch, seq_len)}")
-    if spans is not None and spans.get_device() != at:
+    if spans is not None and spans.device != of_q[0].device:
         raise ValueError(f"spans are on {spans.device}")
     if slopes is not None:
         _check_like("slopes", torch.float32, (n_heads,), at, slopes)
     if lse is not None:
         _check_like("lse", torch.float32, (batch, n_heads, seq_len), at, lse)
-    _check_here(of_q[0])
 
 
 def attention_supported(seq_len: int, head_dim: int) -> bool:
@@ -1076,23 +1046,20 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: int,
     three the sequence may have any length; a row that sees nothing gets zeros and a ``lse`` of -infinity.  Keys of another document
     that share a block of 128 with those of a row have to be finite; padding need not."""
     if spans is not None or softcap != 0.0 or slopes is not None:
+        if q.is_cuda:
+            if spans is not None and (spans.batch != batch or spans.seq != seq_len):
+                raise ValueError(f"spans are of {(spans.batch, spans.seq)}, not of {(batch, seq_len)}")
+            N.launch_count += N.host().attention_masked_fwd(q, k, v, out, lse, None if spans is None else spans._buf, slopes, batch, seq_len,
+                                                            n_heads, n_kv_heads, head_dim, softcap, causal, _status_ptr(q.device))
+            return
         _check_masked((q, out), (k, v), spans, softcap, slopes, lse, batch, seq_len, n_heads, n_kv_heads, head_dim)
         if batch == 0 or seq_len == 0:
             return
-        if not q.is_cuda:
-            q4, k4, v4 = (t.reshape(batch, seq_len, -1, head_dim).float() for t in (q, k, v))
-            o4, l4 = ref_attention_masked(q4, k4, v4, spans.rows if spans is not None else None, causal, softcap, slopes)
-            out.copy_(o4.reshape(batch * seq_len, -1))
-            if lse is not None:
-                lse.copy_(l4)
-            return
-        rows, tiles, _, padded = spans._pointers() if spans is not None else (None, None, None, None)
-        N.check(
-            _fn("attention_masked_fwd")(_at(q), _at(k), _at(v), _at(out), _at(lse), rows, tiles, padded, _at(slopes), batch, seq_len, n_heads,
-                                        n_kv_heads, head_dim, q.stride(0), k.stride(0), v.stride(0), out.stride(0), 1.0 / math.sqrt(head_dim),
-                                        softcap, int(causal), _status_ptr(q.device), _stream()),
-            "attention_masked_fwd",
-        )
+        q4, k4, v4 = (t.reshape(batch, seq_len, -1, head_dim).float() for t in (q, k, v))
+        o4, l4 = ref_attention_masked(q4, k4, v4, spans.rows if spans is not None else None, causal, softcap, slopes)
+        out.copy_(o4.reshape(batch * seq_len, -1))
+        if lse is not None:
+            lse.copy_(l4)
         return
     for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
         _check_2d_bf16(t, name)
@@ -1163,24 +1130,28 @@ def attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Te
 
     ``spans``, ``softcap`` and ``slopes`` as in the forward pass; with any of them sequences have any length, the default
     ``scratch`` is this call's own, and rows that see nothing, or are seen by nobody, get zeros."""
-    masked = spans is not None or softcap != 0.0 or slopes is not None
-    if not masked:
-        for t, name in ((q, "q"), (k, "k"), (v, "v"), (o, "o"), (d_o, "d_o"), (dq, "dq"), (dk, "dk"), (dv, "dv")):
-            _check_2d_bf16(t, name)
-    else:
+    if spans is not None or softcap != 0.0 or slopes is not None:
+        if q.is_cuda:
+            if spans is not None and (spans.batch != batch or spans.seq != seq_len):
+                raise ValueError(f"spans are of {(spans.batch, spans.seq)}, not of {(batch, seq_len)}")
+            N.launch_count += N.host().attention_masked_bwd(
+                q, k, v, o, d_o, lse, dq, dk, dv, scratch, rope, None if spans is None else spans._buf, slopes, batch, seq_len, n_heads, n_kv_heads,
+                head_dim, softcap, causal, _status_ptr(q.device))
+            return
         _check_masked((q, o, d_o, dq), (k, v, dk, dv), spans, softcap, slopes, lse, batch, seq_len, n_heads, n_kv_heads, head_dim)
         if batch == 0 or seq_len == 0:
             return
-        if not q.is_cuda:
-            q4, k4, v4 = (t.detach().reshape(batch, seq_len, -1, head_dim).float().requires_grad_(True) for t in (q, k, v))
-            with torch.enable_grad():
-                o4, _ = ref_attention_masked(q4, k4, v4, spans.rows if spans is not None else None, causal, softcap, slopes)
-            for to, g in zip((dq, dk, dv), torch.autograd.grad(o4, (q4, k4, v4), d_o.reshape(batch, seq_len, -1, head_dim).float())):
-                to.copy_(g.reshape(batch * seq_len, -1))
-            if rope is not None:
-                dq.copy_(ref_rope(dq, rope, seq_len, n_heads, head_dim, backward=True))
-                dk.copy_(ref_rope(dk, rope, seq_len, n_kv_heads, head_dim, backward=True))
-            return
+        q4, k4, v4 = (t.detach().reshape(batch, seq_len, -1, head_dim).float().requires_grad_(True) for t in (q, k, v))
+        with torch.enable_grad():
+            o4, _ = ref_attention_masked(q4, k4, v4, spans.rows if spans is not None else None, causal, softcap, slopes)
+        for to, g in zip((dq, dk, dv), torch.autograd.grad(o4, (q4, k4, v4), d_o.reshape(batch, seq_len, -1, head_dim).float())):
+            to.copy_(g.reshape(batch * seq_len, -1))
+        if rope is not None:
+            dq.copy_(ref_rope(dq, rope, seq_len, n_heads, head_dim, backward=True))
+            dk.copy_(ref_rope(dk, rope, seq_len, n_kv_heads, head_dim, backward=True))
+        return
+    for t, name in ((q, "q"), (k, "k"), (v, "v"), (o, "o"), (d_o, "d_o"), (dq, "dq"), (dk, "dk"), (dv, "dv")):
+        _check_2d_bf16(t, name)
     if not q.is_cuda:
         B, S = batch, seq_len
         q4, k4, v4, do4 = (t.reshape(B, S, -1, head_dim) for t in (q, k, v, d_o))
@@ -1192,15 +1163,14 @@ def attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Te
             dq.copy_(ref_rope(dq, rope, S, n_heads, head_dim, backward=True))
             dk.copy_(ref_rope(dk, rope, S, n_kv_heads, head_dim, backward=True))
         return
-    if seq_len % 128 and not (any_length or masked):
+    if seq_len % 128 and not any_length:
         N.check(-1, "attention_bwd")
     if rope is not None and (rope.dtype != torch.float32 or not rope.is_contiguous() or rope.device != q.device
                              or rope.shape[0] < seq_len or tuple(rope.shape[1:]) != (head_dim // 2, 2)):
         raise ValueError("rope must be the table of the sequence and head dim on the device of q")
+    lib = N.lib()
     need = attention_bwd_scratch_bytes(batch, seq_len, n_heads, n_kv_heads)
-    if scratch is None and masked:
-        scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
-    elif scratch is None:
+    if scratch is None:
         key = (q.device.index, _stream())
         scratch = _attn_scratch.get(key)
         if scratch is None or scratch.numel() < need:
@@ -1209,16 +1179,6 @@ def attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Te
     elif scratch.device != q.device or scratch.dtype != torch.uint8 or scratch.numel() < need or not scratch.is_contiguous():
         raise ValueError(f"scratch must be {need} contiguous bytes on {q.device}")
     scale = 1.0 / math.sqrt(head_dim)
-    if masked:
-        rows, tiles, _, padded = spans._pointers() if spans is not None else (None, None, None, None)
-        N.check(
-            _fn("attention_masked_bwd")(_at(q), _at(k), _at(v), _at(o), _at(d_o), _at(lse), _at(dq), _at(dk), _at(dv), _at(scratch), rows, tiles,
-                                        padded, _at(slopes), batch, seq_len, n_heads, n_kv_heads, head_dim, q.stride(0), k.stride(0), v.stride(0),
-                                        o.stride(0), d_o.stride(0), dq.stride(0), dk.stride(0), dv.stride(0), scale, softcap, int(causal),
-                                        _at(rope), _status_ptr(q.device), _stream()),
-            "attention_masked_bwd", launches=3,
-        )
-        return
     N.check(
         _fn("attention_bwd")(_at(q), _at(k), _at(v), _at(o), _at(d_o), _at(lse), _at(dq), _at(dk), _at(dv), _at(scratch),
                              batch, seq_len, n_heads, n_kv_heads, head_dim, q.stride(0), k.stride(0), v.stride(0), o.stride(0),
