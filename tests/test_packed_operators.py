@@ -227,7 +227,7 @@ def test_refusals_of_masked_attention(device):
     both(heads=(H, 3, D))
     both(heads=(2 * H, 2 * G, 32))
     both(spans=K.attention_spans(torch.zeros(B, S + 1, dtype=torch.int32, device=device)))
-    for cap in (-1.0, math.inf, math.nan):
+    for cap in (-1.0, math.inf, math.nan, 1e-10, 1e31, 1e-50):
         both(softcap=cap)
     both(slopes=torch.zeros(H - 1, device=device))
     both(slopes=torch.zeros(H, device=device).double())

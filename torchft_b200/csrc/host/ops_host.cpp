@@ -50,13 +50,17 @@ struct Args {
   const Tensor& tensor() {
     PyObject* o = next();
     TORCH_CHECK_TYPE(THPVariable_Check(o), "argument ", at, " must be a tensor");
-    return THPVariable_Unpack(o);
+    return with_memory(THPVariable_Unpack(o));
   }
   const Tensor* maybe() {
     PyObject* o = next();
     if (o == Py_None) return nullptr;
     TORCH_CHECK_TYPE(THPVariable_Check(o), "argument ", at, " must be a tensor or None");
-    return &THPVariable_Unpack(o);
+    return &with_memory(THPVariable_Unpack(o));
+  }
+  const Tensor& with_memory(const Tensor& t) const {
+    TORCH_CHECK_TYPE(!t.unsafeGetTensorImpl()->is_python_dispatch(), "argument ", at, " must be a plain tensor, not one whose operators are Python's");
+    return t;
   }
   long long integer() {
     const long long v = PyLong_AsLongLong(next());
@@ -187,8 +191,8 @@ struct Mask {
     causal = a.truth();
     TORCH_CHECK_VALUE((dim == 64 || dim == 128) && heads > 0 && kv_heads > 0 && heads % kv_heads == 0,
                       "masked attention takes head dims 64 and 128 and groups of equally many query heads");
-    TORCH_CHECK_VALUE(c >= 0.0 && c < INFINITY, "softcap must be 0 or a finite cap");
     cap = static_cast<float>(c);
+    TORCH_CHECK_VALUE(c == 0.0 || (cap >= 1e-9f && cap <= 1e30f), "softcap must be 0 or a cap from 1e-9 to 1e30");
   }
   // a [batch * seq, n * dim] view of bf16
   void view(const Tensor& t, const char* name, int n, at::Device device) const {

@@ -57,7 +57,8 @@ struct MaskParams {
     return tiles[(static_cast<long long>(b) * ((seq + 127) / 128) + t) * 2 + which];
   }
 
-  // Keys that the `n` tiles of 128 queries from q0 on look at.
+  // Keys that the `n` tiles of 128 queries from q0 on look at.  (Here and in queries_of the ends are held to the sequence, so that no span, whatever
+  // wrote it, leads outside of it.)
   __device__ __forceinline__ KeyRange keys_of(int b, int q0, int n, int seq) const {
     if (rows == nullptr) return {0, causal ? min(seq, q0 + n * 128) : seq};
     KeyRange r = {INT_MAX, 0};
@@ -66,7 +67,7 @@ struct MaskParams {
       r.lo = min(r.lo, x.x);
       r.hi = max(r.hi, x.y);
     }
-    return r;
+    return {max(r.lo, 0), min(r.hi, seq)};
   }
 
   // Keys that each of the 128 queries from q0 on sees (of those inside the sequence).
@@ -89,7 +90,7 @@ struct MaskParams {
   __device__ __forceinline__ KeyRange queries_of(int b, int t, int seq) const {
     if (rows == nullptr) return {causal ? t * 128 : 0, seq};
     const int4 x = tile(b, t, seq, 1);
-    return {x.x, x.y};
+    return {max(x.x, 0), min(x.y, seq)};
   }
 
   __device__ __forceinline__ RowMask column(int b, int key, int seq) const {
@@ -181,7 +182,7 @@ struct MaskParams {
 
 inline int set_mask(MaskParams* m, const void* rows, const void* tiles, const int* padded, const float* slopes, float scale, float softcap, int causal,
                     int seq) {
-  if ((rows != nullptr) != (tiles != nullptr) || (rows != nullptr) != (padded != nullptr) || !(softcap >= 0.f) || !(softcap < INFINITY))
+  if ((rows != nullptr) != (tiles != nullptr) || (rows != nullptr) != (padded != nullptr) || !(softcap == 0.f || (softcap >= 1e-9f && softcap <= 1e30f)))
     return FTB200_E_BADARG;
   if ((reinterpret_cast<uintptr_t>(rows) & 15) || (reinterpret_cast<uintptr_t>(tiles) & 15)) return FTB200_E_ALIGN;
   if (seq > (1 << 30)) return FTB200_E_TOOBIG;

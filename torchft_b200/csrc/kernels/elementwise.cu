@@ -63,8 +63,8 @@ constexpr int NORM_THREADS = 256;
 
 // out = x * rstd * w ;  optionally first h = x + res (written to h_out) and normalise h.  Bound by memory (by L2 where the
 // rows fit there): every vector is read once, all of a thread's loads are in flight together, and the 256 / TPR rows of
-// a block wait for nothing of each other's.  With a block per row, read twice around three barriers: 63.3 us for
-// 8192 x 4096 (51.8 now, 5.2 TB/s), 32.4 for 8192 x 2048 (28.0), 9.5 for 3000 x 1024 (7.8).
+// a block wait for nothing of each other's.  8192 x 4096 41.3 us (6.5 TB/s), 8192 x 2048 22.3, 3000 x 1024 5.9; with vectors
+// that were loaded word by word 49.5, 26.7, 8.5, and with them and a block per row, read twice around three barriers, 63.3, 32.4, 9.5.
 template <int TPR, int VPT>
 __global__ void __launch_bounds__(NORM_THREADS)
 rmsnorm_fwd_kernel(const bf16x8* x, const bf16x8* res, bf16x8* h_out,
@@ -170,7 +170,9 @@ constexpr int NORM_BWD_THREADS = 512;
 // A group keeps its columns over all its rows, so dw accumulates in registers; the groups of a block meet in shared memory
 // at the end and leave one row of partial sums.  One block per SM, 2 to 16 groups in it: what a row waits for (its loads,
 // its reduction) is covered by the rows of the other groups, which nothing ties to it.  Two rows a block and iteration around one block-wide sum, two blocks per SM, 296 rows of partial sums:
-// 8192 x 2048 45.3 us (38.0 now, both kernels), 3000 x 1024 19.4 (14.0), 2500 x 8192 60.9 (50.7), 8192 x 4096 67.8 (66.8).
+// 8192 x 2048 45.3 us (38.0 in this form, both kernels), 3000 x 1024 19.4 (14.0), 2500 x 8192 60.9 (50.7), 8192 x 4096 67.8 (66.8), all with
+// vectors loaded word by word.  With whole ones 8192 x 2048 34.7 -> 29.2, 3000 x 1024 12.0 -> 10.7, 2500 x 8192 45.4 -> 36.8, 8192 x 4096
+// 62.3 -> 50.7 (5.3 TB/s; replayed from a graph).
 template <int TPR, int VPT>
 __global__ void __launch_bounds__(NORM_BWD_THREADS, 1)
 rmsnorm_bwd_kernel(const bf16x8* dy, const bf16x8* x, const bf16x8* w,
@@ -398,7 +400,7 @@ __global__ void swiglu_bwd_kernel(const __nv_bfloat16* ds, const bf16x8* gu, bf1
 // read a second time from the L2, last pieces first (they are the likeliest still there) and, like the writes, without a claim to
 // stay.  The exponential unit (two an element) and the issue slots come next, hence packed pairs, no one-hot test outside
 // the target's vector, and blocks of 512: three on an SM are seldom all in the same pass, and have the registers for four loads
-// in flight.  8192 x 128256 1015 -> 778 us (5.4 TB/s), 4096 x 50304 221 -> 156, 1024 x 32000 45 -> 35, 750 x 8192 18 -> 14;
+// in flight.  8192 x 128256 1015 -> 778 us (5.4 TB/s), 4096 x 50304 221 -> 156 (142 since its vectors load whole), 1024 x 32000 45 -> 35, 750 x 8192 18 -> 14;
 // in blocks of 1024, two loads, 769, 172, 35, 16; first pieces first 847, 176, 39, 16.
 constexpr int CE_LOADS = 4, CE_THREADS = 512;
 

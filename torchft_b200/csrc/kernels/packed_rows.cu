@@ -18,7 +18,7 @@ namespace {
 //
 // A block takes 1024 tokens, a thread one: scans over the block find each token's document and its prefix's end, and where the first document
 // began before the block or the last one ends behind it, the block looks there itself, 4096 tokens at a time, so that no block waits for another.
-// Bound by latency.
+// Bound by latency: 1 x 8192 tokens 5.2 us, 1 x 16384 5.5, documents of 1000 on average.  (One block a row: 68 us for 16384.)
 constexpr int SPAN_THREADS = 1024;
 constexpr int TILE = 128;
 constexpr int NONE = INT_MAX;
@@ -183,6 +183,7 @@ __global__ void __launch_bounds__(SPAN_THREADS) spans_kernel(const int* document
 //
 // Bound by memory.  A block takes `per_block` tokens: each (token, pair) has its sine taken once, into shared memory, while the first
 // vectors are on their way, and serves all heads.  A thread keeps its place in the head and steps over heads and tokens, without a division.
+// 8192 tokens, 40 of 48 heads of 128 in bf16, three axes: 30 us (5.6 TB/s); with divisions for the places 63.
 constexpr int ROPE_THREADS = 256;
 constexpr int ROPE_LOADS = 4;    // vectors a thread has in flight
 constexpr int ROPE_VECTORS = 8;  // a thread and block, where there are that many

@@ -2,6 +2,7 @@
 
     python -m torchft_b200.ops.bench_kernels gemm --m 8192 --n 8192 --k 8192 --layout fwd
     python -m torchft_b200.ops.bench_kernels adamw --n 1073741824
+    python -m torchft_b200.ops.bench_kernels packed
     python -m torchft_b200.ops.bench_kernels all
 
 Each line printed is JSON: achieved TFLOP/s or GB/s and the fraction of the measured
@@ -240,9 +241,63 @@ def bench_attention(batch: int, seq: int, hq: int, hkv: int, iters: int, compare
     return res
 
 
+def bench_packed(iters: int) -> list:
+    """The operators of packed batches and of layer norm at the shapes of a Llama-3 8B layer: 8192 tokens in documents of
+    1000 on average, 32 query and 8 key/value heads of 128.  Attention counts the pairs that are seen."""
+    dev = "cuda"
+    hbm, tf, how = _peaks()
+    T, D, H, G, HD = 8192, 4096, 32, 8, 128
+    out = []
+
+    def row(name, ms, nbytes=0, flops=0.0):
+        r = {"kernel": name, "ms": ms}
+        if nbytes:
+            r["gbs"] = nbytes / ms / 1e6
+            r[f"frac_of_{how}_copy_bw"] = r["gbs"] / hbm
+        if flops:
+            r["tflops"] = flops / ms / 1e9
+            r[f"frac_of_{how}_cublas_peak"] = r["tflops"] / tf
+        out.append(r)
+
+    gen = torch.Generator().manual_seed(0)
+    documents = (torch.rand(1, T, generator=gen) < 1e-3).cumsum(1).int().to(dev)
+    row("attention_spans", timeit(lambda: K.attention_spans(documents), iters))
+    spans = K.attention_spans(documents)
+    pairs = float((spans.rows[..., 1] - spans.rows[..., 0]).clamp(min=0).sum())
+
+    qkv = (torch.randn(T, (H + 2 * G) * HD, device=dev) * 0.5).bfloat16()
+    q, k, v = qkv[:, : H * HD], qkv[:, H * HD : (H + G) * HD], qkv[:, (H + G) * HD :]
+    o, lse, dqkv = torch.empty(T, H * HD, device=dev, dtype=torch.bfloat16), torch.empty(1, H, T, device=dev), torch.empty_like(qkv)
+    d_o = torch.randn_like(o)
+    dq, dk, dv = dqkv[:, : H * HD], dqkv[:, H * HD : (H + G) * HD], dqkv[:, (H + G) * HD :]
+    slopes = 2.0 ** (-8.0 * (torch.arange(H, device=dev, dtype=torch.float32) + 1) / H)
+    all_pairs = T * (T + 1) / 2
+    for name, n, how_masked in (("documents", pairs, {"spans": spans}), ("documents, cap", pairs, {"spans": spans, "softcap": 50.0}),
+                                ("cap", all_pairs, {"softcap": 50.0}), ("slopes", all_pairs, {"slopes": slopes})):
+        fl = 4.0 * H * HD * n
+        row(f"attention_fwd({name})", timeit(lambda: K.attention_fwd(q, k, v, 1, T, H, G, HD, o, lse, **how_masked), iters), flops=fl)
+        row(f"attention_bwd({name})", timeit(lambda: K.attention_bwd(q, k, v, o, d_o, lse, dq, dk, dv, 1, T, H, G, HD, **how_masked), iters), flops=2.5 * fl)
+
+    bufs = [torch.randn_like(qkv) for _ in range(4)]
+    inv, axis = K.rope_axes_freqs([16, 24, 24], 10000.0, dev)
+    positions = torch.randint(0, T, (3, T), device=dev, dtype=torch.int32)
+    at = iter(range(1 << 30))
+    row("rope_axes", timeit(lambda: K.rope_axes_(bufs[next(at) % 4], positions, inv, axis, H + G, HD), iters), T * (H + G) * HD * 2 * 2)
+
+    xs = [torch.randn(T, D, device=dev).bfloat16() for _ in range(8)]
+    w, b = torch.ones(D, device=dev).bfloat16(), torch.zeros(D, device=dev).bfloat16()
+    y, h, dx = (torch.empty_like(xs[0]) for _ in range(3))
+    _, mean, rstd, _ = K.layernorm_fwd(xs[0], w, b)
+    x = lambda: xs[next(at) % 8]  # noqa: E731
+    row("layernorm_fwd(add+norm)", timeit(lambda: K.layernorm_fwd(x(), w, b, res=x(), h_out=h, out=y), iters), T * D * 2 * 4)
+    row("layernorm_bwd", timeit(lambda: K.layernorm_bwd(x(), x(), w, mean, rstd, dres=x(), dx=dx), iters), T * D * 2 * 4)
+    K.check_status(qkv.device)
+    return out
+
+
 def main() -> None:
     ap = argparse.ArgumentParser()
-    ap.add_argument("what", choices=["gemm", "gemm_gather", "adamw", "rmsnorm", "attention", "elementwise", "all"])
+    ap.add_argument("what", choices=["gemm", "gemm_gather", "adamw", "rmsnorm", "attention", "elementwise", "packed", "all"])
     ap.add_argument("--world", type=int, default=4)
     ap.add_argument("--batch", type=int, default=1)
     ap.add_argument("--seq", type=int, default=8192)
@@ -268,6 +323,9 @@ def main() -> None:
         print(json.dumps(bench_attention(a.batch, a.seq, a.heads, a.kv_heads, a.iters, not a.no_compare, a.head_dim)), flush=True)
     if a.what in ("elementwise", "all"):
         for r in bench_elementwise(a.iters):
+            print(json.dumps(r), flush=True)
+    if a.what in ("packed", "all"):
+        for r in bench_packed(a.iters):
             print(json.dumps(r), flush=True)
     if a.what in ("rmsnorm", "all"):
         print(json.dumps(bench_rmsnorm(8192, 4096, a.iters)), flush=True)

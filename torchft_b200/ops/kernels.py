@@ -869,7 +869,7 @@ class AttentionSpans:
         b = a + 8 * batch * self.n_tiles
         c = b + batch * seq
         self._at = (0, a, b, c, c + batch * ((seq + 1023) // 1024))
-        self._buf = torch.empty(self._at[4], dtype=torch.int32, device=device) if buf is None else buf
+        self._buf = torch.zeros(self._at[4], dtype=torch.int32, device=device) if buf is None else buf  # zeros: nobody sees anything
 
     @property
     def device(self) -> torch.device:
@@ -1000,8 +1000,8 @@ def _check_masked(of_q, of_kv, spans: Optional[AttentionSpans], softcap: float, 
             if t.shape != shape or t.dtype != torch.bfloat16 or t.stride(1) != 1 or t.get_device() != at:
                 raise ValueError(f"a tensor of {heads} heads must be bf16 {shape} with unit inner stride on {of_q[0].device}, got {t.dtype} "
                                  f"{tuple(t.shape)} on {t.device}")
-    if not 0.0 <= softcap < math.inf:
-        raise ValueError("softcap must be 0 or a finite cap")
+    if softcap != 0.0 and not 1e-9 <= softcap <= 1e30:
+        raise ValueError("softcap must be 0 or a cap from 1e-9 to 1e30")
     if spans is not None and (spans.batch, spans.seq) != (batch, seq_len):
         raise ValueError(f"spans are of {(spans.batch, spans.seq)}, not of {(batch, seq_len)}")
     if spans is not None and spans.device != of_q[0].device:
