@@ -65,7 +65,7 @@ __device__ __forceinline__ void group_sums(float (&v)[N], float* part) {
 constexpr int FWD_THREADS = 256;
 
 // Every vector is read once and all of a thread's loads are in flight together, but the variance waits for the mean.  Bound by memory: 8192 x 4096
-// with a residual 43.2 us (6.2 TB/s), 8192 x 2048 23.5, 3000 x 1024 6.8, 64 x 1024 2.4.
+// with a residual 42.9 us (6.3 TB/s), 8192 x 2048 23.3, 2400 x 1024 4.4, 64 x 1024 2.2; in fp32 8192 x 4096 81.5 (6.6 TB/s).
 template <typename T, int TPR, int VPT>
 __global__ void __launch_bounds__(TPR > FWD_THREADS ? TPR : FWD_THREADS)
 layernorm_fwd_kernel(const typename Row<T>::V* x, const typename Row<T>::V* res, typename Row<T>::V* h_out, const typename Row<T>::V* w,
@@ -325,18 +325,23 @@ __global__ void __launch_bounds__(1024) layernorm_columns_kernel(const float* pa
   }
 }
 
-// Threads per row and vectors per thread.  Forward: as few warps a row as 4 vectors a thread allow; with `few` rows, which leave the
-// SMs room, twice the threads and half the vectors.
-template <typename F>
-int fwd_shape(int D8, bool few, F&& f) {
+// Threads per row and vectors per thread.  Forward: 2 vectors a thread, and 4 for more than 4 M elements of bf16 in rows of more than 2048.  With 4
+// instead of 2: 64 x 1024 in bf16 2.9 us instead of 2.2, 2400 x 1024 5.1 (4.4), 600 x 4096 5.3 (4.9), 1200 x 4096 8.8 (8.8), 8192 x 4096 43.1
+// (44.9); in fp32 2400 x 1024 12.2 (9.2), 8192 x 4096 85.5 (81.4), 2400 x 8192 56.4 (54.7).
+template <bool FOUR, typename F>
+int fwd_shape(int D8, bool four, F&& f) {
   auto is = [&](auto tpr, auto vpt) { return f(tpr, vpt); };
 #define FTB200_SHAPE(T, V) is(std::integral_constant<int, T>(), std::integral_constant<int, V>())
   if (D8 <= 32) return FTB200_SHAPE(32, 1);
   if (D8 <= 64) return FTB200_SHAPE(32, 2);
-  if (D8 <= 128) return few ? FTB200_SHAPE(64, 2) : FTB200_SHAPE(32, 4);
-  if (D8 <= 256) return few ? FTB200_SHAPE(128, 2) : FTB200_SHAPE(64, 4);
-  if (D8 <= 512) return few ? FTB200_SHAPE(256, 2) : FTB200_SHAPE(128, 4);
-  if (D8 <= 1024) return few ? FTB200_SHAPE(512, 2) : FTB200_SHAPE(256, 4);
+  if (D8 <= 128) return FTB200_SHAPE(64, 2);
+  if (D8 <= 256) return FTB200_SHAPE(128, 2);
+  if constexpr (FOUR) {
+    if (D8 <= 512 && four) return FTB200_SHAPE(128, 4);
+    if (D8 <= 1024 && four) return FTB200_SHAPE(256, 4);
+  }
+  if (D8 <= 512) return FTB200_SHAPE(256, 2);
+  if (D8 <= 1024) return FTB200_SHAPE(512, 2);
   if (D8 <= 2048) return FTB200_SHAPE(512, 4);
   return FTB200_E_TOOBIG;
 }
@@ -362,7 +367,7 @@ int layernorm_fwd(const void* x, const void* res, void* h_out, const void* w, co
                   int D, float eps, cudaStream_t stream) {
   using V = typename Row<T>::V;
   const int D8 = D / 8;
-  return fwd_shape(D8, rows <= ftb200::sm_count(), [&](auto tpr, auto vpt) -> int {
+  return fwd_shape<sizeof(T) == 2>(D8, rows * D8 > (1 << 19), [&](auto tpr, auto vpt) -> int {
     constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value, THREADS = TPR > FWD_THREADS ? TPR : FWD_THREADS;
     const long long blocks = (rows + THREADS / TPR - 1) / (THREADS / TPR);
     if (blocks > 0x7fffffffLL) return FTB200_E_TOOBIG;
