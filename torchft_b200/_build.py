@@ -197,7 +197,7 @@ def build_host() -> Path:
         ]
         objs = _compile_objects(sources, [torch_dir / "version.py"], ["g++"], flags, "h")  # another torch: compiled again
         if _needs_link(HOST_MOD, objs):
-            libs = ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+            libs = ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python"]
             _run(["g++", "-shared", "-o", str(HOST_MOD), *map(str, objs), f"-L{torch_dir / 'lib'}", *libs])
         return HOST_MOD
 

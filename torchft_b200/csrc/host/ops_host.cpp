@@ -9,6 +9,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -92,9 +93,10 @@ struct Unlocked {
   Unlocked(const Unlocked&) = delete;
 };
 
-Tensor empty(at::IntArrayRef shape, const at::TensorOptions& options) {
+// On a device that has been checked: straight from the allocator (at::empty's way there takes as long again).
+Tensor empty(at::IntArrayRef shape, at::ScalarType type, at::Device device) {
   Unlocked unlocked;
-  return at::empty(shape, options);
+  return Tensor(at::detail::empty_cuda(shape, type, device, std::nullopt));
 }
 
 template <typename F, typename... A>
@@ -158,7 +160,7 @@ PyObject* attention_spans(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   const Stream stream = here(documents);
   const long long B = documents.size(0), S = documents.size(1);
   const SpanParts parts(B, S);
-  Tensor buf = empty({parts.end}, documents.options());
+  Tensor buf = empty({parts.end}, at::kInt, documents.device());
   if (B > 0 && S > 0) {
     TORCH_CHECK_VALUE(B <= INT32_MAX && S <= INT32_MAX, "too many documents");
     int* base = buf.data_ptr<int>();
@@ -268,7 +270,7 @@ PyObject* attention_masked_bwd(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   const long long need = entries.bwd_scratch(m.batch, m.seq, m.heads, m.kv_heads);
   Tensor own;
   if (scratch == nullptr) {
-    own = empty({need}, q.options().dtype(at::kByte));
+    own = empty({need}, at::kByte, device);
     scratch = &own;
   }
   TORCH_CHECK_VALUE(scratch->device() == device && scratch->scalar_type() == at::kByte && scratch->numel() >= need && scratch->is_contiguous(),
@@ -335,8 +337,8 @@ PyObject* pack(std::initializer_list<Tensor> ts) {
 }
 
 // The caller's result or a new one.
-Tensor result(const Tensor* given, at::IntArrayRef shape, const at::TensorOptions& options) {
-  return given != nullptr ? *given : empty(shape, options);
+Tensor result(const Tensor* given, at::IntArrayRef shape, at::ScalarType type, at::Device device) {
+  return given != nullptr ? *given : empty(shape, type, device);
 }
 
 // (x, w, b or None, eps, then res, h_out, out, mean, rstd or None each) -> (out, mean, rstd, h)
@@ -362,9 +364,9 @@ PyObject* layernorm_fwd(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   TORCH_CHECK_VALUE(res == nullptr || h_given == nullptr || out_given == nullptr || h_given->data_ptr() != out_given->data_ptr() || T == 0,
                     "out and h_out are two results");
   const Stream stream = here(x);
-  const auto floats = x.options().dtype(at::kFloat);
-  Tensor out = result(out_given, x.sizes(), x.options()), mean = result(mean_given, {T}, floats), rstd = result(rstd_given, {T}, floats);
-  Tensor h = res == nullptr ? x : result(h_given, x.sizes(), x.options());
+  Tensor out = result(out_given, {T, D}, type, device);
+  Tensor mean = result(mean_given, {T}, at::kFloat, device), rstd = result(rstd_given, {T}, at::kFloat, device);
+  Tensor h = res == nullptr ? x : result(h_given, {T, D}, type, device);
   if (T > 0)
     launch("layernorm_fwd", entries.layernorm_fwd, x.data_ptr(), at_of(res), res == nullptr ? nullptr : h.data_ptr(), w.data_ptr(), at_of(b),
            out.data_ptr(), mean.data_ptr<float>(), rstd.data_ptr<float>(), T, static_cast<int>(D), static_cast<float>(eps), type == at::kFloat,
@@ -397,8 +399,8 @@ PyObject* layernorm_bwd(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   like(&mean, "mean", at::kFloat, {T}, device);
   like(&rstd, "rstd", at::kFloat, {T}, device);
   const Stream stream = here(x);
-  Tensor dx = result(dx_given, x.sizes(), x.options()), dw = result(dw_given, w.sizes(), w.options()), db;
-  if (bias) db = result(db_given, w.sizes(), w.options());
+  Tensor dx = result(dx_given, {T, D}, type, device), dw = result(dw_given, {D}, type, device), db;
+  if (bias) db = result(db_given, {D}, type, device);
   if (T == 0) {
     if (!accumulate) {
       dw.zero_();
@@ -409,7 +411,7 @@ PyObject* layernorm_bwd(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   const long long need = entries.layernorm_scratch(static_cast<int>(D));
   Tensor own;
   if (scratch == nullptr) {
-    own = empty({need}, x.options().dtype(at::kFloat));
+    own = empty({need}, at::kFloat, device);
     scratch = &own;
   }
   TORCH_CHECK_VALUE(scratch->device() == device && scratch->scalar_type() == at::kFloat && scratch->is_contiguous() && scratch->numel() >= need &&

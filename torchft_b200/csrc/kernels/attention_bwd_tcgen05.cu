@@ -894,15 +894,15 @@ int attention_bwd_impl(const void* q, const void* k, const void* v, const void* 
   if (rc == 0) rc = encode_rows(&tdk, dk, batch, seq, static_cast<long long>(n_kv_heads) * D, ld_dk, D / 2, 32);
   if (rc == 0) rc = encode_rows(&tdv, dv, batch, seq, static_cast<long long>(n_kv_heads) * D, ld_dv, D / 2, 32);
   if (rc != 0) return rc;
-  static bool attr_set = false;
-  if (!attr_set) {
+  static std::atomic<unsigned long long> ready{0};  // per device
+  if (!ftb200::once_per_device(ready)) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess)
       return FTB200_E_CUDA;
     // the warpgroups share out what a CTA is launched with: with fewer registers a thread the increase would wait for good
     cudaFuncAttributes attr;
     if (cudaFuncGetAttributes(&attr, kernel) != cudaSuccess) return FTB200_E_CUDA;
     if (attr.numRegs < LAUNCH_REGS) return FTB200_E_REGS;
-    attr_set = true;
+    ftb200::done_on_device(ready);
   }
   const long long pieces = rows * n_heads * (D / 8);
   if ((pieces + 255) / 256 > 0x7fffffffLL) return FTB200_E_TOOBIG;
