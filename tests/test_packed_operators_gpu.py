@@ -173,6 +173,15 @@ def test_large_scores_under_documents(D, G):
     _check(qkv, do, B, S, H, G, D, spans.rows, _run(qkv, do, B, S, H, G, D, spans=spans))
 
 
+@pytest.mark.parametrize("B,S,H,G,D", [(3, 2500, 8, 8, 64), (5000, 40, 1, 1, 64), (37, 129, 10, 5, 128)])
+def test_more_key_blocks_than_fit_the_chip(B, S, H, G, D):
+    """Sorted by their work up to 4096 of them, as they come beyond; of unequal documents, and padding that nobody sees."""
+    ids, _ = _documents(B, S, 300, pad=True, seed=B)
+    spans = K.attention_spans(ids)
+    qkv, do = _packed(B, S, H, G, D, S)
+    _check(qkv, do, B, S, H, G, D, spans.rows, _run(qkv, do, B, S, H, G, D, spans=spans))
+
+
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf, torch.finfo(torch.bfloat16).min])
 @pytest.mark.parametrize("D,G,cap", [(64, 2, 0.0), (128, 1, 0.0), (128, 2, 30.0)])
 def test_padding_may_hold_anything(bad, D, G, cap):

@@ -43,7 +43,7 @@
 // With MASK a key is seen by a range of queries of its own (attention_masks.cuh), so a block walks over the query tiles of that range only, and
 // a softmax thread, whose key it is, holds the range's ends.  With SCORE the scores were capped or lowered by their distance, which is done
 // again here, and dS gets the factor 1 - tanh^2 by way of P, once dV's operand has been made of it.
-// 1 x 8192, 32/8 heads of 128, all four launches: causal with a cap 1308 us (1050 TFLOP/s), with slopes 1208; documents of 1000 tokens on average 315 (588
+// 1 x 8192, 32/8 heads of 128, all three launches: causal with a cap 1315 us (1045 TFLOP/s), with slopes 1190; documents of 1000 tokens on average 311 (595
 // TFLOP/s of the pairs that are seen; their blocks hold 1.3 times as many), of which 43 clear dQ's sums and read O and dO, at the rate of a copy.
 //
 // Every mbarrier wait is bounded; on expiry the CTA records FTB200_ST_TIMEOUT in the caller's
@@ -135,7 +135,47 @@ struct BwdParams {
   const float4* rope;  // null, or (cos, sin) pairs [seq][D / 2]: dQ and dK are rotated back
   int* status;
   ftb200::MaskParams mask;  // of the kernels with MASK
+  const int* order;    // with MASK: null, or the key blocks of all sequences, those that the most queries look at first
 };
+
+// Documents make key blocks unequal, and where a block starts is nothing to go by.  One block of threads sorts them, n_tiles of `batch` sequences, by the
+// query tiles that look at them (counted, from 511 on alike), most first.
+constexpr int MAX_ORDERED = 4096;
+__device__ __forceinline__ void order_key_blocks(const ftb200::MaskParams& mask, int batch, int seq, int* order) {
+  constexpr int BINS = 512;
+  __shared__ int first[BINS];  // of the blocks with 511 - bin query tiles
+  __shared__ int sums[32];
+  const int n_tiles = (seq + 127) / 128, n = batch * n_tiles;
+  const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5;
+  auto bin = [&](int i) {
+    const ftb200::KeyRange r = mask.queries_of(i / n_tiles, i % n_tiles, seq);
+    return BINS - 1 - (r.hi > r.lo ? min((r.hi + 127) / 128 - r.lo / 128, BINS - 1) : 0);
+  };
+  for (int i = tid; i < BINS; i += threads) first[i] = 0;
+  __syncthreads();
+  for (int i = tid; i < n; i += threads) atomicAdd(&first[bin(i)], 1);
+  __syncthreads();
+  const int each = BINS / threads;  // consecutive bins a thread
+  int own = 0;
+  for (int k = 0; k < each; ++k) own += first[tid * each + k];
+  int sum = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += t;
+  }
+  if (lane == 31) sums[warp] = sum;
+  __syncthreads();
+  int at = sum - own;
+  for (int w = 0; w < warp; ++w) at += sums[w];
+  for (int k = 0; k < each; ++k) {
+    const int c = first[tid * each + k];
+    first[tid * each + k] = at;
+    at += c;
+  }
+  __syncthreads();
+  for (int i = tid; i < n; i += threads) order[atomicAdd(&first[bin(i)], 1)] = i;
+}
 
 // Eight elements (four pairs) rotated back by their angles (cos, sin, cos, sin).
 __device__ __forceinline__ void rotate_back(float* f, const float4& c0, const float4& c1) {
@@ -182,10 +222,11 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 
   // early key blocks see the most queries under a causal mask: schedule them first
   const int per_block = p.batch * p.n_kv_heads * p.split;
-  const int jb = static_cast<int>(blockIdx.x) / per_block;
+  int jb = static_cast<int>(blockIdx.x) / per_block;
   const int share = static_cast<int>(blockIdx.x) % p.split;
-  const int bh = static_cast<int>(blockIdx.x) % per_block / p.split;
-  const int b = bh / p.n_kv_heads, hk = bh % p.n_kv_heads;
+  int bh = static_cast<int>(blockIdx.x) % per_block / p.split;
+  int b = bh / p.n_kv_heads;
+  const int hk = bh % p.n_kv_heads;
   const int rep = p.n_heads / p.n_kv_heads / p.split;  // of this CTA
   const int h0 = (hk * p.split + share) * rep;
   const int n_qtiles = (p.seq + BQ - 1) / BQ;
@@ -234,6 +275,12 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 
   ftb200::wait_for_previous();
   if constexpr (MASK) {
+    if (p.order != nullptr) {
+      const int block = p.order[static_cast<int>(blockIdx.x) / (p.n_kv_heads * p.split)];
+      b = block / n_qtiles;
+      jb = block - b * n_qtiles;
+      bh = b * p.n_kv_heads + hk;
+    }
     const ftb200::KeyRange r = p.mask.queries_of(b, jb, p.seq);
     first_q = r.lo / BQ;
     end_q = r.hi > r.lo ? (r.hi + BQ - 1) / BQ : first_q;
@@ -675,9 +722,11 @@ __global__ void __launch_bounds__(256) attention_bwd_prep_kernel(const __nv_bflo
                                                                  const float* lse, float* neg_lse2,
                                                                  float* neg_delta, float4* dq_acc,
                                                                  int seq, int n_heads, long long pieces, long long ld_o,
-                                                                 long long ld_do, float scale) {
+                                                                 long long ld_do, float scale, const ftb200::MaskParams mask, int* order,
+                                                                 int batch) {
   ftb200::wait_for_previous();
   ftb200::start_next();
+  if (order != nullptr && blockIdx.x == 0) order_key_blocks(mask, batch, seq, order);
   constexpr int LANES = D / 8;
   const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
   const bool live = i < pieces;
@@ -859,14 +908,14 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 }  // namespace
 
-// Scratch the backward pass needs, in bytes: fp32 dQ accumulator, -scale delta, -log2(e) lse, and the shares' dV and dK where the
-// query heads are shared out.  (sized for head dim 128; enough for 64 as well)
+// Scratch the backward pass needs, in bytes: fp32 dQ accumulator, -scale delta, -log2(e) lse, the shares' dV and dK where the
+// query heads are shared out, and under a mask the order of the key blocks.  (sized for head dim 128; enough for 64 as well)
 FTB200_API long long ftb200_attention_bwd_scratch_bytes(int batch, int seq, int n_heads, int n_kv_heads) {
   if (batch <= 0 || seq <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0) return 0;
   const long long tiles = (static_cast<long long>(seq) + BQ - 1) / BQ, rows = batch * tiles * BQ;
   const long long ctas = batch * tiles * n_kv_heads;
   const int split = head_split(ctas, n_heads / n_kv_heads);
-  return rows * n_heads * 128 * 4 + 2 * rows * n_heads * 4 + (split > 1 ? ctas * split * (2 * 128 * BKV * 4) : 0);
+  return rows * n_heads * 128 * 4 + 2 * rows * n_heads * 4 + (split > 1 ? ctas * split * (2 * 128 * BKV * 4) : 0) + MAX_ORDERED * 4;
 }
 
 namespace {
@@ -904,11 +953,16 @@ int attention_bwd_impl(const void* q, const void* k, const void* v, const void* 
     if (attr.numRegs < LAUNCH_REGS) return FTB200_E_REGS;
     ftb200::done_on_device(ready);
   }
+  // Where the chip takes more than two CTAs an SM one after another.  (512 CTAs, documents of 1000 on average, four draws: 0, 10, 0 and 5 % of a
+  // training pass; 192 CTAs: the sorting adds 1 us and nothing is gained.)  Without a mask of ranges the early blocks see the most.
+  const bool ordered = MASK && mask.rows != nullptr && batch * tiles <= MAX_ORDERED && batch * tiles * n_kv_heads * split > 2LL * ftb200::sm_count();
+  float* parts = neg_lse2 + rows * n_heads;
+  int* order = reinterpret_cast<int*>(parts + (split > 1 ? batch * tiles * n_kv_heads * split * (2LL * D * BKV) : 0));
   const long long pieces = rows * n_heads * (D / 8);
   if ((pieces + 255) / 256 > 0x7fffffffLL) return FTB200_E_TOOBIG;
   ftb200::launch_after(attention_bwd_prep_kernel<D>, static_cast<unsigned>((pieces + 255) / 256), 256, 0, stream,
       reinterpret_cast<const __nv_bfloat16*>(o), reinterpret_cast<const __nv_bfloat16*>(d_o), lse, neg_lse2, neg_delta,
-      reinterpret_cast<float4*>(dq_acc), seq, n_heads, pieces, ld_o, ld_do, scale);
+      reinterpret_cast<float4*>(dq_acc), seq, n_heads, pieces, ld_o, ld_do, scale, mask, ordered ? order : nullptr, batch);
   BwdParams p = {};
   p.batch = batch; p.seq = seq; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads; p.causal = causal;
   p.scale = scale; p.scale_log2 = scale * 1.4426950408889634f;
@@ -918,7 +972,8 @@ int attention_bwd_impl(const void* q, const void* k, const void* v, const void* 
   p.rope = reinterpret_cast<const float4*>(cos_sin);
   p.split = split;
   p.mask = mask;
-  p.dkv_part = reinterpret_cast<float4*>(neg_lse2 + rows * n_heads);
+  p.order = ordered ? order : nullptr;
+  p.dkv_part = reinterpret_cast<float4*>(parts);
   const long long grid = static_cast<long long>(batch) * n_kv_heads * tiles * split;
   if (grid > 0x7fffffffLL) return FTB200_E_TOOBIG;
   ftb200::launch_after(kernel, static_cast<unsigned>(grid), NUM_THREADS, SMEM_BYTES, stream, tq, tk, tv, tdo, tdk,

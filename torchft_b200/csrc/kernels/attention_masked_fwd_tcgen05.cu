@@ -32,7 +32,7 @@
 // next sequence's); keys there are in no query's range, queries there are not stored.
 //
 // 1 x 8192, 32/8 heads of 128: documents of 1000 tokens on average 113 us (658 TFLOP/s of the pairs that are seen), with a cap 147; causal with a
-// cap 603 (912 TFLOP/s; 434 in the kernel without masks and caps), with slopes 551 (659 with the first block first).
+// cap 603 (912 TFLOP/s; 434 in the kernel without masks and caps), with slopes 525 (659 with the first block first).
 //
 // Every mbarrier wait is bounded; on expiry the CTA records FTB200_ST_TIMEOUT in the caller's status word, frees its TMEM and returns.
 #include <cuda.h>
