@@ -513,3 +513,62 @@ def test_threads_with_streams_of_their_own():
                 assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
                 # dQ is summed by atomics, as above
                 assert (got[2].double() - want[2].double()).norm() / want[2].double().norm() < U
+
+
+def test_attention_without_a_log_sum_exp():
+    B, S, H, G, D = 2, 200, 4, 1, 128
+    ids, _ = _documents(B, S, 50, pad=True)
+    spans = K.attention_spans(ids)
+    qkv, do = _packed(B, S, H, G, D, 4)
+    q, k, v = _parts(qkv, H, G, D)
+    out, want = torch.empty_like(do), torch.empty_like(do)
+    K.attention_fwd(q, k, v, B, S, H, G, D, out, spans=spans)
+    K.attention_fwd(q, k, v, B, S, H, G, D, want, torch.empty(B, H, S, device="cuda"), spans=spans)
+    assert torch.equal(out, want)
+
+
+def test_attention_offsets_beyond_32_bits():
+    """3.4 G elements of Q, K and V, 2.3 G of dQ: the last document against the same one by itself, where every tile and block begins alike."""
+    S, H, G, D, last = 560000 // 128 * 128, 32, 8, 128, 640
+    if torch.cuda.get_device_properties(0).total_memory < 60e9:
+        pytest.skip("needs 60 GB")
+    ids = (torch.arange(S, device="cuda") // 1000).to(torch.int32)
+    ids[S - last :] = 1 << 20
+    qkv = torch.zeros(S, (H + 2 * G) * D, dtype=torch.bfloat16, device="cuda")
+    do = torch.zeros(S, H * D, dtype=torch.bfloat16, device="cuda")
+    small, do_small = _packed(1, last, H, G, D, 1)
+    qkv[S - last :], do[S - last :] = small, do_small
+    out, lse, d = _run_no_check(qkv, do, 1, S, H, G, D, spans=K.attention_spans(ids.view(1, S)))
+    o1, l1, d1 = _run_no_check(small, do_small, 1, last, H, G, D, spans=K.attention_spans(ids[S - last :].view(1, last)))
+    K.check_status(qkv.device)
+    assert torch.equal(out[S - last :], o1) and torch.equal(lse[..., S - last :], l1)
+    assert not out[: S - last].any() and not d[: S - last].any()
+    kv = slice(H * D, None)
+    # dK and dV of a group in one sum or in four (few blocks by themselves are shared out); dQ by atomics: a rounding more of each
+    torch.testing.assert_close(d[S - last :, kv].double(), d1[:, kv].double(), rtol=2 * U, atol=2.0**-12)
+    torch.testing.assert_close(d[S - last :, : H * D].double(), d1[:, : H * D].double(), rtol=2 * U, atol=2.0**-12)
+
+
+def test_rows_beyond_32_bits():
+    T, D = 530000, 4096
+    x = torch.zeros(T, D, dtype=torch.bfloat16, device="cuda")
+    x[-300:] = torch.randn(300, D, device="cuda").to(torch.bfloat16)
+    w, b = torch.randn(2, D, device="cuda").to(torch.bfloat16)
+    y, mean, rstd, _ = K.layernorm_fwd(x, w, b)
+    y1, mean1, rstd1, _ = K.layernorm_fwd(x[-300:], w, b)
+    # two shapes of threads: an element goes through at most 32 + 8 additions in either, each off by 2^-24 of sums up to mean |x| < 1 (of squares: of
+    # their own sum, halved in rstd); y is rounded once more, or one step apart
+    torch.testing.assert_close(mean[-300:], mean1, rtol=0, atol=80 * 2.0**-24)
+    torch.testing.assert_close(rstd[-300:], rstd1, rtol=80 * 2.0**-24, atol=0)
+    torch.testing.assert_close(y[-300:], y1, rtol=2 * U, atol=2 * U * 1e-2)
+    assert torch.equal(y[: T - 300], b.expand(T - 300, D))
+    dx, _, db = K.layernorm_bwd(x, x, w, mean, rstd, dx=y)
+    dx1, _, db1 = K.layernorm_bwd(x[-300:], x[-300:], w, mean[-300:], rstd[-300:])
+    assert torch.equal(dx[-300:], dx1) and not dx[: T - 300].any()
+    # each column's 300 values, of any order
+    torch.testing.assert_close(db, db1, rtol=2 * U, atol=300 * 2.0**-24 * float(x[-300:].float().abs().sum(0).max()))
+    inv, axis = K.rope_axes_freqs([32, 32], 1e4, "cuda")
+    at = torch.randint(0, 1 << 20, (2, T), dtype=torch.int32, device="cuda")
+    want = K.rope_axes_(x[-300:].clone(), at[:, -300:].contiguous(), inv, axis, 32, 128)
+    K.rope_axes_(x, at, inv, axis, 32, 128)
+    assert torch.equal(x[-300:], want) and not x[: T - 300].any()
