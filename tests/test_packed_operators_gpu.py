@@ -173,7 +173,7 @@ def test_large_scores_under_documents(D, G):
     _check(qkv, do, B, S, H, G, D, spans.rows, _run(qkv, do, B, S, H, G, D, spans=spans))
 
 
-@pytest.mark.parametrize("B,S,H,G,D", [(3, 2500, 8, 8, 64), (5000, 40, 1, 1, 64), (37, 129, 10, 5, 128)])
+@pytest.mark.parametrize("B,S,H,G,D", [(3, 2500, 8, 8, 64), (5000, 40, 1, 1, 64), (37, 129, 10, 5, 128), (40, 300, 6, 2, 64), (1, 2000, 64, 8, 128)])
 def test_more_key_blocks_than_fit_the_chip(B, S, H, G, D):
     """Sorted by their work up to 4096 of them, as they come beyond; of unequal documents, and padding that nobody sees."""
     ids, _ = _documents(B, S, 300, pad=True, seed=B)
