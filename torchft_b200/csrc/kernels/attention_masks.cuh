@@ -8,12 +8,10 @@
 //
 //   y = log2(e) (softcap tanh(scale s / softcap) - slope |query - key|)
 //
-// tanh(x) is x P(x^2), of degree 2 up to |x| = 0.35 and of degree 4 up to 0.8 (relative errors of 2.9e-6 and 1.0e-6; least largest error, by Lawson's
-// iteration of weighted least squares): four or six operations of the FMA pipe, with scale and cap inside the coefficients, while the
+// tanh(x) is x P(x^2), of degree 3 up to |x| = 0.4 (a relative error of 9.8e-8) and of degree 5 up to 0.8 (5.8e-8; least largest error, by
+// Lawson's iteration of weighted least squares): five or seven operations of the FMA pipe, with scale and cap inside the coefficients, while the
 // exponential unit, which the softmax wants for itself, stays free.  A warp's scores that go beyond take 1 - 2 / (exp(2x) + 1), with an error
-// of about 1e-7 of the cap, which is what counts in a score.  At a cap of 50 a score is off by 5e-5 at most, and a probability by as much of itself, a
-// fortieth of half a step of the bf16 that it is rounded to.  (A degree more each, up to 0.4 and 0.8, errors of 1e-7 and 6e-8: 4 x 2048 tokens in documents of
-// 400 on average, 32/8 heads of 64, forward 88.2 us instead of 84.8, 2 x 4096, heads of 128, a cap of 30: 208 instead of 198.)
+// of about 1e-7 of the cap, which is what counts in a score.
 #pragma once
 
 #include <limits.h>
@@ -49,7 +47,7 @@ struct MaskParams {
   int capped;
   const float* slopes;  // null, or [heads]
   float scale_log2;     // log2(e) scale
-  float near[3], poly[5];  // of s^2: y = s P(s^2)
+  float near[4], poly[6];  // of s^2: y = s P(s^2)
   float near_up_to, poly_up_to;  // |s| that they hold for
   float cap2;           // log2(e) softcap
   float in2;            // 2 log2(e) scale / softcap
@@ -167,9 +165,9 @@ struct MaskParams {
         big[(c >> 1) & 3] = fmaxf(fmaxf(big[(c >> 1) & 3], fabsf(__uint_as_float(sv[c]))), fabsf(__uint_as_float(sv[c + 1])));
       const float most = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
       if (__all_sync(0xffffffffu, most <= near_up_to)) {
-        by_polynomial<N, 3>(sv, near);
+        by_polynomial<N, 4>(sv, near);
       } else if (__all_sync(0xffffffffu, most <= poly_up_to)) {
-        by_polynomial<N, 5>(sv, poly);
+        by_polynomial<N, 6>(sv, poly);
       } else {
 #pragma unroll
         for (int c = 0; c < N; ++c)
@@ -197,17 +195,18 @@ inline int set_mask(MaskParams* m, const void* rows, const void* tiles, const in
   m->capped = softcap > 0.f;
   m->scale_log2 = static_cast<float>(scale * LOG2E);
   if (softcap > 0.f) {
-    constexpr double P[5] = {0.9999989943440225, -0.3332537195890023, 0.1323056553360009, -0.04918014148907632, 0.012100138385891959};
-    constexpr double NEAR[3] = {0.9999971307655218, -0.33290954112874505, 0.1239503130076369};
+    constexpr double P[6] = {0.9999999420836679, -0.333326749210523, 0.1332104829082429, -0.05311431573861419, 0.01909330062970014,
+                             -0.004355299563624438};
+    constexpr double NEAR[4] = {0.9999999019017232, -0.33331362461616354, 0.132709767765151, -0.04755360368917723};
     const double k = static_cast<double>(scale) / softcap, cap2 = softcap * LOG2E;
     double power = cap2 * k;
     bool fits = true;
-    for (int i = 0; i < 5; ++i, power *= k * k) {
-      if (i < 3) m->near[i] = static_cast<float>(NEAR[i] * power);
+    for (int i = 0; i < 6; ++i, power *= k * k) {
+      if (i < 4) m->near[i] = static_cast<float>(NEAR[i] * power);
       m->poly[i] = static_cast<float>(P[i] * power);
       fits = fits && isfinite(m->poly[i]);
     }
-    m->near_up_to = fits ? static_cast<float>(0.35 / k) : -1.f;
+    m->near_up_to = fits ? static_cast<float>(0.4 / k) : -1.f;
     m->poly_up_to = fits ? static_cast<float>(0.8 / k) : -1.f;
     m->cap2 = static_cast<float>(cap2);
     m->in2 = static_cast<float>(2.0 * LOG2E * k);
