@@ -70,6 +70,7 @@ constexpr int SOFTMAX_WARPS = 8;
 constexpr int DRAIN_WARPS = 4;
 // Registers: a CTA is launched with 128 a thread (65536 / 512, checked on the host) and shares them out by warpgroup:
 // TMA and MMA issue, drain (128 elements of dQ^T in flight), two of softmax (a thread keeps 64 probabilities).
+// Each role ends by itself, so that no value is held across a change of shares, and the kernels with MASK keep nothing in local memory (checked too).
 constexpr int LAUNCH_REGS = 128, ISSUE_REGS = 48, DRAIN_REGS = 144, SOFTMAX_REGS = 160;
 static_assert(ISSUE_REGS + DRAIN_REGS + 2 * SOFTMAX_REGS <= 4 * LAUNCH_REGS, "more registers than the CTA is launched with");
 constexpr int CPT = BQ / 2;        // query columns per softmax thread: two threads per key row
@@ -391,7 +392,7 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       const bool padded = MASK && p.mask.has_padding(b, p.seq, lane);
       TileWalk next{h0, first_q};  // the tile whose Q or dO is waited for
       auto clear = [&](uint32_t off, int tile) {
-        if (padded) p.mask.clear_padding(smem + off, SLABS, b, tile * 128, p.seq, lane);
+        if (padded) p.mask.clear_padding(smem_base + off, SLABS, b, tile * 128, p.seq, lane);
       };
       bool ok = (!MASK || T > 0) && wait(BAR_KV, 0) && wait(BAR_Q_FULL, 0);
       if (ok) {
@@ -436,6 +437,14 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       }
       if (ok && elect_one()) umma_commit(bar(BAR_DKV_DONE));
       __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+      tc_fence_after();
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"(TMEM_COLS) : "memory");
+    } else if (warp == 2 && lane == 0 && *abort_flag && p.status != nullptr) {
+      atomicExch(p.status, FTB200_ST_TIMEOUT);
     }
   } else if (warp < 8) {
     // ---------------- dQ drain: TMEM lane = head-dim index ----------------
@@ -482,6 +491,8 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     __syncwarp();
+    tc_fence_before();
+    __syncthreads();
   } else {
     // ---------------- softmax, dK/dV store ----------------
     regs_inc<SOFTMAX_REGS>();
@@ -513,26 +524,25 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       const ulonglong2* delta2 = lse2 + BQ / 4;
       float pe[CPT];
       if constexpr (SCORE) {
-        uint32_t sv[CPT];
-        tmem_ld32(s_addr, sv);
-        tmem_ld32(s_addr + 32, sv + 32);
-        tmem_wait_ld();
-        p.mask.cap_scores<CPT>(sv);
+        uint32_t sv[32];
         const float slope2 = p.mask.slope2(w.h);
         const float far = static_cast<float>(w.qt * BQ + g * CPT - (jb * BKV + row));
-        const bool all = mine.all(w.qt * BQ, BQ);
+        const bool all = __all_sync(0xffffffffu, mine.all(w.qt * BQ, BQ));  // the same in all lanes; said so, as whole warps access tensor memory below
         const unsigned long long inv2 = f2_pack(p.mask.neg_inv_cap2_sq, p.mask.neg_inv_cap2_sq), one2 = f2_pack(1.f, 1.f);
         auto probabilities = [&](auto partial) {
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const int q0 = w.qt * BQ + g * CPT + half * 32;
             const uint32_t bits = decltype(partial)::value ? ftb200::range_bits(mine.lo - q0, mine.hi - q0) : 0u;
+            tmem_ld32(s_addr + half * 32, sv);  // (with both halves in registers two words of a thread would go to local memory)
+            tmem_wait_ld();
+            p.mask.cap_scores<32>(sv);
             uint32_t pt[16];
 #pragma unroll
             for (int c = 0; c < 16; ++c) {
               const int qi = half * 32 + 2 * c;
               const ulonglong2 l4 = lse2[qi / 4];
-              const unsigned long long y = f2_pack(__uint_as_float(sv[qi]), __uint_as_float(sv[qi + 1]));
+              const unsigned long long y = f2_pack(__uint_as_float(sv[2 * c]), __uint_as_float(sv[2 * c + 1]));
               float x0, x1;
               f2_unpack(f2_add(y, c % 2 == 0 ? l4.x : l4.y), x0, x1);
               if (p.mask.slopes != nullptr) {
@@ -578,7 +588,7 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         }
       }
       if constexpr (MASK) {
-        if (!SCORE && !mine.all(w.qt * BQ, BQ)) {
+        if (!SCORE && !__all_sync(0xffffffffu, mine.all(w.qt * BQ, BQ))) {
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const int q0 = w.qt * BQ + g * CPT + half * 32;
@@ -702,14 +712,8 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       // the shared memory has been read; elect_one may take another lane, so all wait for what they have committed
       bulk_wait_read();
     }
-  }
-
-  tc_fence_before();
-  __syncthreads();
-  if (threadIdx.x == 0 && *abort_flag && p.status != nullptr) atomicExch(p.status, FTB200_ST_TIMEOUT);
-  if (warp == 1) {
-    tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+    tc_fence_before();
+    __syncthreads();
   }
 }
 
@@ -950,7 +954,7 @@ int attention_bwd_impl(const void* q, const void* k, const void* v, const void* 
     // the warpgroups share out what a CTA is launched with: with fewer registers a thread the increase would wait for good
     cudaFuncAttributes attr;
     if (cudaFuncGetAttributes(&attr, kernel) != cudaSuccess) return FTB200_E_CUDA;
-    if (attr.numRegs < LAUNCH_REGS) return FTB200_E_REGS;
+    if (attr.numRegs < LAUNCH_REGS || (MASK && attr.localSizeBytes != 0)) return FTB200_E_REGS;
     ftb200::done_on_device(ready);
   }
   // Where the chip takes more than two CTAs an SM one after another.  (512 CTAs, documents of 1000 on average, four draws: 0, 10, 0 and 5 % of a

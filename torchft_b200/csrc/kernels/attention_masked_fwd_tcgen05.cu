@@ -52,8 +52,9 @@ constexpr int TILES = 2;   // tiles per item
 constexpr int BKV = 128;   // keys per block
 constexpr int NUM_THREADS = 384;
 // Registers: a CTA is launched with 168 a thread (65536 / 384, checked on the host); the first warpgroup gives most of its own to the two
-// softmax warpgroups: 72 + 2 * 216 = 3 * 168.
-constexpr int LAUNCH_REGS = 168, ISSUE_REGS = 72, SOFTMAX_REGS = 216;
+// softmax warpgroups: 40 + 2 * 232 = 3 * 168.  With these shares nothing is kept in local memory (checked on the host too), and each role ends by
+// itself, so that no value is held across a change of shares: what a role needs at its end it reads again.
+constexpr int LAUNCH_REGS = 168, ISSUE_REGS = 40, SOFTMAX_REGS = 232;
 static_assert(ISSUE_REGS + 2 * SOFTMAX_REGS <= 3 * LAUNCH_REGS, "more registers than the CTA is launched with");
 constexpr int ROW_WARPS = 4;                  // softmax warps per tile
 constexpr int READERS = 2 + TILES * ROW_WARPS;  // warps that read an item
@@ -275,7 +276,7 @@ attention_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
         const bool padded = p.mask.has_padding(it.batch, p.seq, lane);
         // what stands in padding reaches neither the products nor the choice of a way for the scores
         auto clear = [&](uint32_t off, int r) {
-          if (padded) p.mask.clear_padding(smem + off, C::SLABS, it.batch, r, p.seq, lane);
+          if (padded) p.mask.clear_padding(smem_base + off, C::SLABS, it.batch, r, p.seq, lane);
         };
         auto issue_s = [&](int t, int j) {
           const int g = blocks + j, st = g % C::STAGES;
@@ -312,7 +313,7 @@ attention_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
           }
           if (j == 0 && full > 0 && !wait(BAR_O_FREE + t, full - 1)) return false;
           const uint32_t vb = same(v_lo + st * STAGE16);
-#pragma unroll
+#pragma unroll 1
           for (int half = 0; half < 2; ++half) {
             if (!wait((half == 0 ? BAR_P_HALF : BAR_P_FULL) + t, g)) return false;
             tc_fence_after();
@@ -388,6 +389,14 @@ attention_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
       }
     }
     __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+      tc_fence_after();
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"(TMEM_COLS) : "memory");
+    } else if (warp == 2 && lane == 0 && *abort_flag && p.status != nullptr) {
+      atomicExch(p.status, FTB200_ST_TIMEOUT);
+    }
   } else {
     // ---------------- softmax + output: one thread per query row ----------------
     regs_inc<SOFTMAX_REGS>();
@@ -414,6 +423,7 @@ attention_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
       const ftb200::KeyRange mine = p.mask.row(it.batch, query, p.seq);
       float slope2 = 0.f;
       if constexpr (SCORE) slope2 = p.mask.slope2(head);
+      __syncwarp();
       float m_used = -INFINITY, l_sum = 0.f;
       for (int j = 0; j < it.blocks; ++j) {
         const int g = blocks + j;
@@ -479,6 +489,7 @@ attention_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
           m_used = m_new;
           l_sum *= alpha;
         }
+        __syncwarp();  // tensor memory is accessed by whole warps
         // O, and P where it has columns of its own, may only be touched once P V of the previous block is done; P V of this block waits for P
         if ((any_raise || C::OWN_P) && g > 0) {
           if (!(ok = wait(BAR_O_DONE + t, g - 1))) break;
@@ -580,14 +591,8 @@ attention_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
     }
     if (lane == 0) bulk_wait_read();
     __syncwarp();
-  }
-
-  tc_fence_before();
-  __syncthreads();
-  if (threadIdx.x == 0 && *abort_flag && p.status != nullptr) atomicExch(p.status, FTB200_ST_TIMEOUT);
-  if (warp == 1) {
-    tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+    tc_fence_before();
+    __syncthreads();
   }
 }
 
@@ -629,7 +634,7 @@ int launch(const Maps& m, const Params& p, long long grid, cudaStream_t stream) 
     // warpgroups would wait for registers that nobody has.
     cudaFuncAttributes attr;
     if (cudaFuncGetAttributes(&attr, kernel) != cudaSuccess) return FTB200_E_CUDA;
-    if (attr.numRegs < LAUNCH_REGS) return FTB200_E_REGS;
+    if (attr.numRegs < LAUNCH_REGS || attr.localSizeBytes != 0) return FTB200_E_REGS;
     ftb200::done_on_device(ready);
   }
   ftb200::launch_after(kernel, static_cast<unsigned>(grid), NUM_THREADS, Cfg<D>::SMEM_BYTES, stream, m.q, m.k, m.v, m.o, p);

@@ -122,12 +122,12 @@ struct MaskParams {
   // Of a tile in shared memory (slabs of 128 rows x 128 bytes; its first row is row `first` of the sequence) the rows that belong to padding
   // become zeros, by one warp: what stands in padding may be anything, and zero times infinity would reach the tile's other rows.  The
   // products that follow see it.
-  __device__ __forceinline__ void clear_padding(uint8_t* tile_mem, int slabs, int b, int first, int seq, int lane) const {
+  __device__ __forceinline__ void clear_padding(uint32_t tile_addr, int slabs, int b, int first, int seq, int lane) const {
     for (int r = lane; r < 128 && first + r < seq; r += 32) {
-      const int4 x = rows[static_cast<long long>(b) * seq + first + r];
-      if (x.y > x.x) continue;
-      for (int s = 0; s < slabs; ++s)
-        for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(tile_mem + s * (128 * 128) + r * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+      const KeyRange x = row(b, first + r, seq);
+      if (x.hi > x.lo) continue;
+      const uint32_t at = tile_addr + r * 128;
+      for (int c = 0; c < slabs * 8; ++c) tc::st_shared_zero16(at + (c >> 3) * (128 * 128) + (c & 7) * 16);
     }
     tc::fence_async_smem();
     __syncwarp();
@@ -171,7 +171,7 @@ struct MaskParams {
       } else {
 #pragma unroll
         for (int c = 0; c < N; ++c)
-          sv[c] = __float_as_uint(fmaf(-2.f * cap2, __frcp_rn(exp2f(__uint_as_float(sv[c]) * in2) + 1.f), cap2));
+          sv[c] = __float_as_uint(fmaf(-2.f * cap2, tc::rcp_approx(exp2f(__uint_as_float(sv[c]) * in2) + 1.f), cap2));
       }
     } else {
 #pragma unroll

@@ -32,8 +32,8 @@ ERRORS = {
     -3: "driver entry point unavailable / tensor-map encode failed",
     -4: "size beyond the supported maximum",
     -5: "CUDA launch error",
-    -6: "the kernel was compiled with fewer registers a thread than its warpgroups share out (a debug build, or another "
-        "compiler)",
+    -6: "the kernel was compiled with fewer registers a thread than its warpgroups share out, or with some in local memory "
+        "(a debug build, or another compiler)",
     E_LIST: "tensors of a list share memory or have none",
 }
 
