@@ -28,3 +28,42 @@ def test_the_masked_attention_kernels_keep_nothing_in_local_memory(tmp_path):
     masked = fwd + [r for r in bwd if "ELb1E" in r[0]]
     assert len(masked) == 8
     assert all(r[1:] == ("0", "0", "0") for r in masked), masked
+
+
+# ------------------------------------------------------------------ padding
+
+
+def _packed(B, S, H, G, D, seed):
+    g = torch.Generator().manual_seed(seed)
+    qkv = torch.randn(B * S, (H + 2 * G) * D, generator=g).to(torch.bfloat16)
+    return qkv, torch.randn(B * S, H * D, generator=g).to(torch.bfloat16)
+
+
+def _parts(t, H, G, D):
+    return t[:, : H * D], t[:, H * D : (H + G) * D], t[:, (H + G) * D :]
+
+
+def _both(qkv, do, B, S, H, G, D, **how):
+    out, lse, d = torch.full_like(do, 7.0), torch.full((B, H, S), 7.0), torch.full_like(qkv, 7.0)
+    K.attention_fwd(*_parts(qkv, H, G, D), B, S, H, G, D, out, lse, **how)
+    K.attention_bwd(*_parts(qkv, H, G, D), out, do, lse, *_parts(d, H, G, D), B, S, H, G, D, **how)
+    return out, lse, d
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf, torch.finfo(torch.bfloat16).min])
+@pytest.mark.parametrize("cap,slopes", [(0.0, None), (20.0, None), (0.0, 0.25)])
+def test_padding_may_hold_anything(bad, cap, slopes):
+    B, S, H, G, D = 2, 64, 4, 2, 64
+    qkv, do = _packed(B, S, H, G, D, 5)
+    ids = (torch.arange(S).expand(B, S) // 13).to(torch.int32).contiguous()
+    ids[:, 40:] = -1
+    ids[1, 7:9] = -2
+    how = {"spans": K.attention_spans(ids), "softcap": cap, "slopes": None if slopes is None else torch.full((H,), slopes)}
+    dead = (ids < 0).view(-1)
+    clean = _both(qkv, do, B, S, H, G, D, **how)
+    qkv[dead], do[dead] = bad, bad
+    dirty = _both(qkv, do, B, S, H, G, D, **how)
+    for x, y in zip(clean, dirty):
+        assert torch.equal(x, y)
+    assert not dirty[0][dead].any() and not dirty[2][dead].any()
+    assert (dirty[1].transpose(1, 2)[ids < 0] == -math.inf).all()

@@ -966,9 +966,12 @@ def attention_spans(documents: torch.Tensor, prefix: Optional[torch.Tensor] = No
 
 def ref_attention_masked(q, k, v, rows=None, causal=True, softcap=0.0, slopes=None):
     """``(out, lse)`` of attention under a mask, in the type of the arguments: 4-D q, k, v as :func:`ref_attention`, ``rows`` as in
-    :class:`AttentionSpans`."""
+    :class:`AttentionSpans`.  What stands in padding reaches neither the others nor, as a gradient, padding."""
     B, S, Hq, Dh = q.shape
     rep = Hq // k.shape[2]
+    if rows is not None:
+        live = (rows[..., 1] > rows[..., 0])[..., None, None]
+        q, k, v = (torch.where(live, t, 0.0) for t in (q, k, v))
     q, k, v = q.transpose(1, 2), k.transpose(1, 2).repeat_interleave(rep, 1), v.transpose(1, 2).repeat_interleave(rep, 1)
     s = q @ k.transpose(-1, -2) / math.sqrt(Dh)
     if softcap > 0:
@@ -985,8 +988,10 @@ def ref_attention_masked(q, k, v, rows=None, causal=True, softcap=0.0, slopes=No
     top = torch.where(top > -math.inf, top, 0.0)
     p = torch.exp(s - top)
     total = p.sum(-1, keepdim=True)
-    o = (p @ v) / torch.where(total > 0, total, 1.0)
-    return o.transpose(1, 2), (top + total.log()).squeeze(-1).detach()
+    o = ((p @ v) / torch.where(total > 0, total, 1.0)).transpose(1, 2)
+    if rows is not None:
+        o = torch.where(live, o, 0.0)  # with it the gradient that comes back
+    return o, (top + total.log()).squeeze(-1).detach()
 
 
 def _check_masked(of_q, of_kv, spans: Optional[AttentionSpans], softcap: float, slopes: Optional[torch.Tensor], lse: Optional[torch.Tensor],
