@@ -49,7 +49,6 @@
 // Every mbarrier wait is bounded; on expiry the CTA records FTB200_ST_TIMEOUT in the caller's
 // status word, frees its TMEM and returns.
 #include <cuda.h>
-#include <cudaTypedefs.h>
 #include <math.h>
 
 #include <initializer_list>
@@ -58,6 +57,7 @@
 #include "attention_masks.cuh"
 #include "ftb200_common.cuh"
 #include "tcgen05_helpers.cuh"
+#include "tensor_maps.cuh"
 
 namespace {
 
@@ -876,38 +876,6 @@ int head_split(long long ctas, int rep) {
   return split;
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static bool tried = false;
-  if (!tried) {
-    tried = true;
-    void* sym = nullptr;
-    cudaDriverEntryPointQueryResult qres;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &qres) == cudaSuccess &&
-        qres == cudaDriverEntryPointSuccess) {
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(sym);
-    }
-  }
-  return fn;
-}
-
-// [batch, seq, cols] bf16 view with row stride ld (elements); box = 64 columns x 128 rows, 128-byte swizzle (dK, dV: half a head x 32 rows, the
-// swizzle as wide as the box)
-int encode_rows(CUtensorMap* map, const void* base, long long batch, long long seq, long long cols, long long ld, unsigned box_cols = 64,
-                unsigned box_rows = 128) {
-  auto fn = encode_fn();
-  if (fn == nullptr) return FTB200_E_DRIVER;
-  cuuint64_t gdim[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(seq), static_cast<cuuint64_t>(batch)};
-  cuuint64_t gstride[2] = {static_cast<cuuint64_t>(ld) * 2, static_cast<cuuint64_t>(seq) * ld * 2};
-  cuuint32_t box[3] = {box_cols, box_rows, 1u};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), gdim, gstride, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : FTB200_E_DRIVER;
-}
-
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace
@@ -940,12 +908,12 @@ int attention_bwd_impl(const void* q, const void* k, const void* v, const void* 
   const int split = head_split(batch * tiles * n_kv_heads, n_heads / n_kv_heads);
   if (rows > 0x7fffffffLL) return FTB200_E_TOOBIG;
   CUtensorMap tq, tk, tv, tdo, tdk, tdv;
-  int rc = encode_rows(&tq, q, batch, seq, static_cast<long long>(n_heads) * D, ld_q);
-  if (rc == 0) rc = encode_rows(&tdo, d_o, batch, seq, static_cast<long long>(n_heads) * D, ld_do);
-  if (rc == 0) rc = encode_rows(&tk, k, batch, seq, static_cast<long long>(n_kv_heads) * D, ld_k);
-  if (rc == 0) rc = encode_rows(&tv, v, batch, seq, static_cast<long long>(n_kv_heads) * D, ld_v);
-  if (rc == 0) rc = encode_rows(&tdk, dk, batch, seq, static_cast<long long>(n_kv_heads) * D, ld_dk, D / 2, 32);
-  if (rc == 0) rc = encode_rows(&tdv, dv, batch, seq, static_cast<long long>(n_kv_heads) * D, ld_dv, D / 2, 32);
+  int rc = ftb200::encode_rows(&tq, q, batch, seq, static_cast<long long>(n_heads) * D, ld_q);
+  if (rc == 0) rc = ftb200::encode_rows(&tdo, d_o, batch, seq, static_cast<long long>(n_heads) * D, ld_do);
+  if (rc == 0) rc = ftb200::encode_rows(&tk, k, batch, seq, static_cast<long long>(n_kv_heads) * D, ld_k);
+  if (rc == 0) rc = ftb200::encode_rows(&tv, v, batch, seq, static_cast<long long>(n_kv_heads) * D, ld_v);
+  if (rc == 0) rc = ftb200::encode_rows(&tdk, dk, batch, seq, static_cast<long long>(n_kv_heads) * D, ld_dk, D / 2, 32);
+  if (rc == 0) rc = ftb200::encode_rows(&tdv, dv, batch, seq, static_cast<long long>(n_kv_heads) * D, ld_dv, D / 2, 32);
   if (rc != 0) return rc;
   static std::atomic<unsigned long long> ready{0};  // per device
   if (!ftb200::once_per_device(ready)) {

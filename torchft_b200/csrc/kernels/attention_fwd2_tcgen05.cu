@@ -36,11 +36,11 @@
 // Every mbarrier wait is bounded; on expiry the CTA records FTB200_ST_TIMEOUT in the caller's
 // status word, frees its TMEM and returns.
 #include <cuda.h>
-#include <cudaTypedefs.h>
 #include <math.h>
 
 #include "ftb200_common.cuh"
 #include "tcgen05_helpers.cuh"
+#include "tensor_maps.cuh"
 
 namespace {
 
@@ -460,35 +460,6 @@ attention_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
   }
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn2() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static bool tried = false;
-  if (!tried) {
-    tried = true;
-    void* sym = nullptr;
-    cudaDriverEntryPointQueryResult qres;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &qres) == cudaSuccess &&
-        qres == cudaDriverEntryPointSuccess) {
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(sym);
-    }
-  }
-  return fn;
-}
-
-// [batch, seq, cols] bf16 view with row stride ld (elements); box = 64 columns x 128 rows (O: 32), 128-byte swizzle
-int encode_rows2(CUtensorMap* map, const void* base, long long batch, long long seq, long long cols, long long ld, unsigned box_rows = 128) {
-  auto fn = encode_fn2();
-  if (fn == nullptr) return FTB200_E_DRIVER;
-  cuuint64_t gdim[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(seq), static_cast<cuuint64_t>(batch)};
-  cuuint64_t gstride[2] = {static_cast<cuuint64_t>(ld) * 2, static_cast<cuuint64_t>(seq) * ld * 2};
-  cuuint32_t box[3] = {64u, box_rows, 1u};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), gdim, gstride, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : FTB200_E_DRIVER;
-}
-
 template <int D, int POLY>
 int launch_fwd2(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to, const Attn2Params& p, long long grid,
                 cudaStream_t stream) {
@@ -527,10 +498,10 @@ FTB200_API int ftb200_attention_fwd2(const void* q, const void* k, const void* v
       (ld_o & 7))
     return FTB200_E_ALIGN;
   CUtensorMap tq, tk, tv, to;
-  int rc = encode_rows2(&tq, q, batch, seq, static_cast<long long>(n_heads) * head_dim, ld_q);
-  if (rc == 0) rc = encode_rows2(&tk, k, batch, seq, static_cast<long long>(n_kv_heads) * head_dim, ld_k);
-  if (rc == 0) rc = encode_rows2(&tv, v, batch, seq, static_cast<long long>(n_kv_heads) * head_dim, ld_v);
-  if (rc == 0) rc = encode_rows2(&to, o, batch, seq, static_cast<long long>(n_heads) * head_dim, ld_o, 32);
+  int rc = ftb200::encode_rows(&tq, q, batch, seq, static_cast<long long>(n_heads) * head_dim, ld_q);
+  if (rc == 0) rc = ftb200::encode_rows(&tk, k, batch, seq, static_cast<long long>(n_kv_heads) * head_dim, ld_k);
+  if (rc == 0) rc = ftb200::encode_rows(&tv, v, batch, seq, static_cast<long long>(n_kv_heads) * head_dim, ld_v);
+  if (rc == 0) rc = ftb200::encode_rows(&to, o, batch, seq, static_cast<long long>(n_heads) * head_dim, ld_o, 64, 32);
   if (rc != 0) return rc;
   Attn2Params p;
   p.batch = batch; p.seq = seq; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads; p.causal = causal;

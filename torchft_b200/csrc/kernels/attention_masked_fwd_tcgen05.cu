@@ -36,12 +36,12 @@
 //
 // Every mbarrier wait is bounded; on expiry the CTA records FTB200_ST_TIMEOUT in the caller's status word, frees its TMEM and returns.
 #include <cuda.h>
-#include <cudaTypedefs.h>
 #include <math.h>
 
 #include "attention_masks.cuh"
 #include "ftb200_common.cuh"
 #include "tcgen05_helpers.cuh"
+#include "tensor_maps.cuh"
 
 namespace {
 
@@ -596,30 +596,6 @@ attention_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
   }
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-    void* sym = nullptr;
-    cudaDriverEntryPointQueryResult qres;
-    const bool found = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &qres) == cudaSuccess &&
-                       qres == cudaDriverEntryPointSuccess;
-    return found ? reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(sym) : nullptr;
-  }();
-  return fn;
-}
-
-// [batch, seq, cols] bf16 view with row stride ld (elements); box = 64 columns x box_rows, 128-byte swizzle
-int encode_rows(CUtensorMap* map, const void* base, long long batch, long long seq, long long cols, long long ld, unsigned box_rows) {
-  auto fn = encode_fn();
-  if (fn == nullptr) return FTB200_E_DRIVER;
-  cuuint64_t gdim[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(seq), static_cast<cuuint64_t>(batch)};
-  cuuint64_t gstride[2] = {static_cast<cuuint64_t>(ld) * 2, static_cast<cuuint64_t>(seq) * ld * 2};
-  cuuint32_t box[3] = {64u, box_rows, 1u};
-  cuuint32_t estr[3] = {1, 1, 1};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : FTB200_E_DRIVER;
-}
-
 struct Maps {
   CUtensorMap q, k, v, o;
 };
@@ -661,10 +637,10 @@ FTB200_API int ftb200_attention_masked_fwd(const void* q, const void* k, const v
   Params p = {};
   Maps m;
   int rc = ftb200::set_mask(&p.mask, rows, tiles, padded, slopes, scale, softcap, causal, seq);
-  if (rc == 0) rc = encode_rows(&m.q, q, batch, seq, static_cast<long long>(n_heads) * head_dim, ld_q, 128);
-  if (rc == 0) rc = encode_rows(&m.k, k, batch, seq, static_cast<long long>(n_kv_heads) * head_dim, ld_k, 128);
-  if (rc == 0) rc = encode_rows(&m.v, v, batch, seq, static_cast<long long>(n_kv_heads) * head_dim, ld_v, 128);
-  if (rc == 0) rc = encode_rows(&m.o, o, batch, seq, static_cast<long long>(n_heads) * head_dim, ld_o, 32);
+  if (rc == 0) rc = ftb200::encode_rows(&m.q, q, batch, seq, static_cast<long long>(n_heads) * head_dim, ld_q);
+  if (rc == 0) rc = ftb200::encode_rows(&m.k, k, batch, seq, static_cast<long long>(n_kv_heads) * head_dim, ld_k);
+  if (rc == 0) rc = ftb200::encode_rows(&m.v, v, batch, seq, static_cast<long long>(n_kv_heads) * head_dim, ld_v);
+  if (rc == 0) rc = ftb200::encode_rows(&m.o, o, batch, seq, static_cast<long long>(n_heads) * head_dim, ld_o, 64, 32);
   if (rc != 0) return rc;
   p.batch = batch; p.seq = seq; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads;
   p.scale_log2 = scale * 1.4426950408889634f;

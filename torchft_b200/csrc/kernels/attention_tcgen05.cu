@@ -24,11 +24,11 @@
 // Every mbarrier wait is bounded; on expiry the CTA records FTB200_ST_TIMEOUT in the
 // caller's status word, frees its TMEM and returns.
 #include <cuda.h>
-#include <cudaTypedefs.h>
 #include <math.h>
 
 #include "ftb200_common.cuh"
 #include "tcgen05_helpers.cuh"
+#include "tensor_maps.cuh"
 
 namespace {
 
@@ -374,35 +374,6 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap tmK,
   }
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static bool tried = false;
-  if (!tried) {
-    tried = true;
-    void* sym = nullptr;
-    cudaDriverEntryPointQueryResult qres;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &qres) == cudaSuccess &&
-        qres == cudaDriverEntryPointSuccess) {
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(sym);
-    }
-  }
-  return fn;
-}
-
-// [rows, cols] bf16 view with row stride ld (elements); box = 64 columns x box_rows rows, 128-byte swizzle
-int encode_rows(CUtensorMap* map, const void* base, long long rows, long long cols, long long ld, int box_rows) {
-  auto fn = encode_fn();
-  if (fn == nullptr) return FTB200_E_DRIVER;
-  cuuint64_t gdim[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
-  cuuint64_t gstride[1] = {static_cast<cuuint64_t>(ld) * 2};
-  cuuint32_t box[2] = {64u, static_cast<cuuint32_t>(box_rows)};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), gdim, gstride, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : FTB200_E_DRIVER;
-}
-
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace
@@ -422,8 +393,8 @@ FTB200_API int ftb200_attention_fwd(const void* q, const void* k, const void* v,
     return FTB200_E_ALIGN;
   CUtensorMap tk, tv;
   const long long rows = static_cast<long long>(batch) * seq;
-  int rc = encode_rows(&tk, k, rows, static_cast<long long>(n_kv_heads) * D, ld_k, BKV);
-  if (rc == 0) rc = encode_rows(&tv, v, rows, static_cast<long long>(n_kv_heads) * D, ld_v, BKV);
+  int rc = ftb200::encode_2d(&tk, k, rows, static_cast<long long>(n_kv_heads) * D, ld_k, 64, BKV);
+  if (rc == 0) rc = ftb200::encode_2d(&tv, v, rows, static_cast<long long>(n_kv_heads) * D, ld_v, 64, BKV);
   if (rc != 0) return rc;
   static bool attr_set = false;
   if (!attr_set) {

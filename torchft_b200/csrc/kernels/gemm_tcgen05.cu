@@ -21,10 +21,10 @@
 // wait expires the CTA raises a shared abort flag, records FTB200_ST_TIMEOUT in the
 // caller's status word, drains, frees its TMEM and returns.
 #include <cuda.h>
-#include <cudaTypedefs.h>
 
 #include "ftb200_common.cuh"
 #include "tcgen05_helpers.cuh"
+#include "tensor_maps.cuh"
 
 namespace {
 
@@ -291,36 +291,6 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
   }
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static bool tried = false;
-  if (!tried) {
-    tried = true;
-    void* sym = nullptr;
-    cudaDriverEntryPointQueryResult qres;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &qres) == cudaSuccess &&
-        qres == cudaDriverEntryPointSuccess) {
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(sym);
-    }
-  }
-  return fn;
-}
-
-// rows x cols bf16 matrix, `cols` contiguous, row stride `ld` elements; box = box_cols x box_rows.
-int encode_2d(CUtensorMap* map, const void* base, long long rows, long long cols, long long ld, int box_cols,
-              int box_rows) {
-  auto fn = get_encode_fn();
-  if (fn == nullptr) return FTB200_E_DRIVER;
-  cuuint64_t gdim[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
-  cuuint64_t gstride[1] = {static_cast<cuuint64_t>(ld) * 2};
-  cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), gdim, gstride, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : FTB200_E_DRIVER;
-}
-
 }  // namespace
 
 // C[M,N] (+)= A * B^T with A logical [M,K], B logical [N,K].
@@ -339,14 +309,14 @@ FTB200_API int ftb200_gemm_bf16(const void* A, const void* B, void* C, int M, in
   CUtensorMap tmA, tmB;
   int rc;
   if (!a_mn_major)
-    rc = encode_2d(&tmA, A, M, K, lda, BK, BM);
+    rc = ftb200::encode_2d(&tmA, A, M, K, lda, BK, BM);
   else
-    rc = encode_2d(&tmA, A, K, M, lda, 64, BK);
+    rc = ftb200::encode_2d(&tmA, A, K, M, lda, 64, BK);
   if (rc) return rc;
   if (!b_mn_major)
-    rc = encode_2d(&tmB, B, N, K, ldb, BK, BN);
+    rc = ftb200::encode_2d(&tmB, B, N, K, ldb, BK, BN);
   else
-    rc = encode_2d(&tmB, B, K, N, ldb, 64, BK);
+    rc = ftb200::encode_2d(&tmB, B, K, N, ldb, 64, BK);
   if (rc) return rc;
 
   static bool attr_set = false;

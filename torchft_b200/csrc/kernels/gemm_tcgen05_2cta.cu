@@ -37,10 +37,10 @@
 #include <algorithm>
 #include <atomic>
 #include <cuda.h>
-#include <cudaTypedefs.h>
 
 #include "ftb200_common.cuh"
 #include "tcgen05_helpers.cuh"
+#include "tensor_maps.cuh"
 
 namespace {
 
@@ -973,35 +973,6 @@ gemv_bf16_kernel(const ftb200::bf16x8* a, const ftb200::bf16x8* B, __nv_bfloat16
   }
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static bool tried = false;
-  if (!tried) {
-    tried = true;
-    void* sym = nullptr;
-    cudaDriverEntryPointQueryResult qres;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &qres) == cudaSuccess &&
-        qres == cudaDriverEntryPointSuccess) {
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(sym);
-    }
-  }
-  return fn;
-}
-
-int encode_2d(CUtensorMap* map, const void* base, long long rows, long long cols, long long ld, int box_cols,
-              int box_rows) {
-  auto fn = get_encode_fn();
-  if (fn == nullptr) return FTB200_E_DRIVER;
-  cuuint64_t gdim[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
-  cuuint64_t gstride[1] = {static_cast<cuuint64_t>(ld) * 2};
-  cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), gdim, gstride, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : FTB200_E_DRIVER;
-}
-
 }  // namespace
 
 // Same arguments as ftb200_gemm_bf16; pairs of CTAs cooperate on 256x256 tiles.
@@ -1121,20 +1092,20 @@ static int launch_2cta(const void* A, const void* B, long long lda, long long ld
   CUtensorMap tmA, tmB, tmC, tmAux;
   int rc;
   if (!p.a_mn)
-    rc = encode_2d(&tmA, A, p.M, p.K, lda, BK, BM);
+    rc = ftb200::encode_2d(&tmA, A, p.M, p.K, lda, BK, BM);
   else
-    rc = encode_2d(&tmA, A, p.K, p.M, lda, 64, BK);
+    rc = ftb200::encode_2d(&tmA, A, p.K, p.M, lda, 64, BK);
   if (rc) return rc;
   if (!p.b_mn)
-    rc = encode_2d(&tmB, B, p.N, p.K, ldb, BK, BN / 2);
+    rc = ftb200::encode_2d(&tmB, B, p.N, p.K, ldb, BK, BN / 2);
   else
-    rc = encode_2d(&tmB, B, p.K, p.N, ldb, 64, BK);
+    rc = ftb200::encode_2d(&tmB, B, p.K, p.N, ldb, 64, BK);
   if (rc) return rc;
   tmC = tmAux = tmA;  // not used without tma_out
   if (p.tma_out) {
-    if (p.C != nullptr) rc = encode_2d(&tmC, p.C, p.M, p.N, p.ldc, 64, 32);
+    if (p.C != nullptr) rc = ftb200::encode_2d(&tmC, p.C, p.M, p.N, p.ldc, 64, 32);
     if (rc == 0 && p.aux != nullptr)
-      rc = encode_2d(&tmAux, p.aux, p.M, EPI == EPI_DSWIGLU ? 2 * p.N : p.N / 2, p.ld_aux, 64, 32);
+      rc = ftb200::encode_2d(&tmAux, p.aux, p.M, EPI == EPI_DSWIGLU ? 2 * p.N : p.N / 2, p.ld_aux, 64, 32);
     if (rc) return rc;
   }
   if (prepare_2cta<BN, SPLIT, EPI>() != cudaSuccess) return FTB200_E_CUDA;
