@@ -113,3 +113,12 @@ def run(tmp_path_factory):
 def test_first_calls_of_several_threads(run, name):
     """None of them sees another's search for the driver's entry point half done."""
     assert run(name, "threads") == [0, 0, 0, 0]
+
+
+@pytest.mark.parametrize("name", ENTRIES)
+def test_attributes_are_set_on_every_device(run, name):
+    """A kernel's limit of shared memory belongs to a device: set once on each that is used, and not at every call."""
+    first, other, again, back, third = run(name, "devices")
+    assert first[0] == other[0] == third[0] > 0  # of each device
+    assert again[0] == other[0] and back[0] == first[0]
+    assert again[1] == 2 * other[1] and back[1] == 2 * first[1] and first[1] > 0

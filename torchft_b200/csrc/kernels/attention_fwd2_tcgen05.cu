@@ -463,8 +463,8 @@ attention_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
 template <int D, int POLY>
 int launch_fwd2(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to, const Attn2Params& p, long long grid,
                 cudaStream_t stream) {
-  static bool attr_set = false;
-  if (!attr_set) {
+  static std::atomic<unsigned long long> ready{0};  // per device
+  if (!ftb200::once_per_device(ready)) {
     if (cudaFuncSetAttribute(attention_fwd2_kernel<D, POLY>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              Cfg<D>::SMEM_BYTES) != cudaSuccess)
       return FTB200_E_CUDA;
@@ -473,7 +473,7 @@ int launch_fwd2(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap&
     cudaFuncAttributes attr;
     if (cudaFuncGetAttributes(&attr, attention_fwd2_kernel<D, POLY>) != cudaSuccess) return FTB200_E_CUDA;
     if (attr.numRegs < LAUNCH_REGS) return FTB200_E_REGS;
-    attr_set = true;
+    ftb200::done_on_device(ready);
   }
   ftb200::launch_after(attention_fwd2_kernel<D, POLY>, static_cast<unsigned>(grid), NUM_THREADS, Cfg<D>::SMEM_BYTES, stream,
       tq, tk, tv, to, p);

@@ -396,11 +396,11 @@ FTB200_API int ftb200_attention_fwd(const void* q, const void* k, const void* v,
   int rc = ftb200::encode_2d(&tk, k, rows, static_cast<long long>(n_kv_heads) * D, ld_k, 64, BKV);
   if (rc == 0) rc = ftb200::encode_2d(&tv, v, rows, static_cast<long long>(n_kv_heads) * D, ld_v, 64, BKV);
   if (rc != 0) return rc;
-  static bool attr_set = false;
-  if (!attr_set) {
+  static std::atomic<unsigned long long> ready{0};  // per device
+  if (!ftb200::once_per_device(ready)) {
     if (cudaFuncSetAttribute(attention_fwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess)
       return FTB200_E_CUDA;
-    attr_set = true;
+    ftb200::done_on_device(ready);
   }
   AttnParams p;
   p.batch = batch; p.seq = seq; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads; p.causal = causal;

@@ -319,12 +319,12 @@ FTB200_API int ftb200_gemm_bf16(const void* A, const void* B, void* C, int M, in
     rc = ftb200::encode_2d(&tmB, B, K, N, ldb, 64, BK);
   if (rc) return rc;
 
-  static bool attr_set = false;
-  if (!attr_set) {
+  static std::atomic<unsigned long long> ready{0};  // per device
+  if (!ftb200::once_per_device(ready)) {
     if (cudaFuncSetAttribute(gemm_bf16_tcgen05_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) !=
         cudaSuccess)
       return FTB200_E_CUDA;
-    attr_set = true;
+    ftb200::done_on_device(ready);
   }
   GemmParams p;
   p.M = M; p.N = N; p.K = K;

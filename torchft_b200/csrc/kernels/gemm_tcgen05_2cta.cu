@@ -1001,11 +1001,11 @@ struct GatherSpec {
 
 template <int BN, bool SPLIT, int EPI>
 static cudaError_t prepare_2cta() {
-  static std::atomic<bool> done{false};
-  if (done.load(std::memory_order_acquire)) return cudaSuccess;
+  static std::atomic<unsigned long long> ready{0};  // per device
+  if (ftb200::once_per_device(ready)) return cudaSuccess;
   const cudaError_t e = cudaFuncSetAttribute(gemm_bf16_tcgen05_2cta_kernel<BN, SPLIT, EPI>,
                                              cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<BN, EPI>::SMEM_BYTES);
-  if (e == cudaSuccess) done.store(true, std::memory_order_release);
+  if (e == cudaSuccess) ftb200::done_on_device(ready);
   return e;
 }
 
