@@ -41,3 +41,79 @@ def test_layernorm_bwd_of_many_rows_a_group(T, D, dtype, use_res):
     for got, terms in ((dw, dyd * xh), (db, dyd)):
         s = terms.sum(0)
         assert ((got.double() - s).abs() <= u * s.abs() + (chain + 2 * e) * terms.abs().sum(0)).all()
+
+
+# ------------------------------------------------------------------ capped scores
+
+
+def _spread(B, S, H, G, D, most, seed):
+    """Queries whose scores go from a few units to `most`, small and large ones next to each other; keys and values of size one."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda n: torch.randn(B, S, n, D, device="cuda", generator=g)  # noqa: E731
+    size = torch.exp(torch.rand(B, S, H, 1, device="cuda", generator=g) * math.log(most)) / 3
+    return (r(H) * size).bfloat16(), r(G).bfloat16(), r(G).bfloat16(), r(H).bfloat16()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("cap,most", [(50.0, 100.0), (250.0, 500.0), (400.0, 50.0), (400.0, 800.0), (1000.0, 100.0), (1000.0, 2000.0), (1e6, 1000.0)])
+def test_caps_of_every_size(cap, most, D):
+    """A score is off by 2^-20 of itself (its product's fp32 sum 2^-22, the cap's form 2^-21) and 2^-21 of caps up to 260, whose large scores take the
+    form of exponentials; a probability by that and, in the backward pass, by three roundings of the log-sum-exp."""
+    B, S, H, G = 1, 300, 4, 2
+    q, k, v, do = _spread(B, S, H, G, D, most, 1)
+    flat = lambda t: t.reshape(B * S, -1)  # noqa: E731
+    out, lse = torch.empty_like(flat(q)), torch.empty(B, H, S, device="cuda")
+    grads = [torch.empty_like(flat(t)) for t in (q, k, v)]
+    K.attention_fwd(flat(q), flat(k), flat(v), B, S, H, G, D, out, lse, softcap=cap)
+    K.attention_bwd(flat(q), flat(k), flat(v), out, flat(do), lse, *grads, B, S, H, G, D, softcap=cap)
+    K.check_status(q.device)
+
+    u = 2.0**-8
+    q, k, v, do = (t.double().transpose(1, 2) for t in (q, k, v, do))
+    k, v = k.repeat_interleave(H // G, 1), v.repeat_interleave(H // G, 1)
+    scale = D**-0.5
+    t = torch.tanh(q @ k.transpose(-1, -2) * scale / cap)
+    s = (cap * t).masked_fill(~torch.ones(S, S, dtype=torch.bool, device="cuda").tril(), -math.inf)
+    want_lse = torch.logsumexp(s, -1)
+    # a product's fp32 sum is off by its terms' size, not its own
+    sizes = (q.abs() @ k.abs().transpose(-1, -2)).clamp(max=1e30) * scale
+    off = 2.0**-21 * (torch.minimum(sizes * (1 - t * t) + (cap * t).abs(), sizes)).amax(-1) + 2.0**-21 * min(cap, 260.0)
+    assert ((lse.double() - want_lse).abs() <= off + 2.0**-20 * want_lse.abs() + 1e-6).all()
+    p = torch.exp(s - want_lse[..., None])
+    o = p @ v
+    four = lambda t: t.reshape(B, S, -1, D).transpose(1, 2).double()  # noqa: E731
+    e_p = 2 * off[..., None]
+    e_o = u * (p @ v.abs() + o.abs()) * 1.05 + 2 * e_p * (p @ v.abs())
+    assert ((four(out) - o).abs() <= e_o + 1e-6).all()
+    delta, dp, f = (do * o).sum(-1, keepdim=True), do @ v.transpose(-1, -2), 1 - t * t
+    e_pb = 2 * (off + 2.0**-21 * want_lse.abs())[..., None]
+    ds = p * (dp - delta) * f * scale
+    e_ds = u * ds.abs() + p * scale * (f * (do.abs() * e_o).sum(-1, keepdim=True) + (dp - delta).abs() * (e_pb * f + 2.0**-19))
+    shared = lambda t: t.view(B, G, H // G, S, D).sum(2)  # noqa: E731
+    back = lambda t: t.transpose(-1, -2)  # noqa: E731
+    for what, got, want, bound in (("dq", grads[0], ds @ k, e_ds @ k.abs()), ("dk", grads[1], shared(back(ds) @ q), shared(back(e_ds) @ q.abs())),
+                                   ("dv", grads[2], shared(back(p) @ do), shared(back(p * (u + e_pb)) @ do.abs()))):
+        wrong = (four(got) - want).abs() / (1.05 * (bound + u * want.abs()) + 1e-6)
+        assert (wrong <= 1).all(), (what, float(wrong.max()))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("size", [0.05, 1.0])
+@pytest.mark.parametrize("cap", [1e12, 1e20, 1e30])
+def test_caps_and_scores_beyond_sense(cap, size, D):
+    """Scores below and about the cap, whose squares are no fp32 numbers any more."""
+    B, S, H, G = 1, 200, 2, 1
+    q, k, v, _ = _spread(B, S, H, G, D, 10.0, 2)
+    q = q * size
+    q, k = (q.double() * cap**0.5).bfloat16(), (k.double() * cap**0.5).bfloat16()
+    flat = lambda t: t.reshape(B * S, -1)  # noqa: E731
+    out, lse = torch.empty_like(flat(q)), torch.empty(B, H, S, device="cuda")
+    K.attention_fwd(flat(q), flat(k), flat(v), B, S, H, G, D, out, lse, softcap=cap)
+    K.check_status(q.device)
+    q, k = q.double().transpose(1, 2), k.double().transpose(1, 2).repeat_interleave(H // G, 1)
+    s = (cap * torch.tanh(q @ k.transpose(-1, -2) * D**-0.5 / cap)).masked_fill(~torch.ones(S, S, dtype=torch.bool, device="cuda").tril(), -math.inf)
+    sizes = (q.abs() @ k.abs().transpose(-1, -2)).amax(-1) * D**-0.5
+    assert out.isfinite().all()
+    # the largest score, to 2^-21 of its terms and 2^-20 of itself
+    want = torch.logsumexp(s, -1)
+    assert ((lse.double() - want).abs() <= 2.0**-21 * sizes + 2.0**-20 * want.abs()).all()

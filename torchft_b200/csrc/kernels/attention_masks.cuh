@@ -12,8 +12,14 @@
 // Lawson's iteration of weighted least squares): five or seven operations of the FMA pipe, with scale and cap inside the coefficients, while the
 // exponential unit, which the softmax wants for itself, stays free.  A warp's scores that go beyond take 1 - 2 / (exp(2x) + 1), with an error
 // of about 1e-7 of the cap, which is what counts in a score.
+//
+// From a cap of about 260 on (head dim 128; of 380 at 64) the last coefficients, the smaller the higher the power of the cap that they are
+// divided by, are no normal numbers any more.  There the short form is taken as far as those that it lost would not be seen, and beyond it scores are
+// scaled first and each takes the form that its own size asks for: 1e-7 of such a cap would be seen in a small score that shares a warp with a
+// large one.  (Scores of a few units under a cap of 1000 take a tenth more time than under one of 50, both passes of 1 x 8192, 32/8 heads of 128.)
 #pragma once
 
+#include <float.h>
 #include <limits.h>
 #include <math.h>
 
@@ -49,9 +55,11 @@ struct MaskParams {
   float scale_log2;     // log2(e) scale
   float near[4], poly[6];  // of s^2: y = s P(s^2)
   float near_up_to, poly_up_to;  // |s| that they hold for
+  int wide;              // a cap beyond that: poly are of scale s / softcap, and hold up to wide_up_to
+  float unit, wide_up_to;
   float cap2;           // log2(e) softcap
   float in2;            // 2 log2(e) scale / softcap
-  float neg_inv_cap2_sq;  // -1 / cap2^2: 1 - tanh^2 = 1 + y^2 times this
+  float neg_inv_cap2_sq;  // -1 / cap2^2: 1 - tanh^2 = 1 + y^2 times this (zero for caps that no product of sense reaches, from 6e18 on)
 
   __device__ __forceinline__ int4 tile(int b, int t, int seq, int which) const {
     return tiles[(static_cast<long long>(b) * ((seq + 127) / 128) + t) * 2 + which];
@@ -155,27 +163,55 @@ struct MaskParams {
     }
   }
 
+  __device__ __forceinline__ float by_exponential(float s) const { return fmaf(-2.f * cap2, tc::rcp_approx(exp2f(s * in2) + 1.f), cap2); }
+
+  __device__ __forceinline__ float by_scaled_polynomial(float s) const {
+    const float x = s * unit, u = x * x;
+    float y = poly[5];
+#pragma unroll
+    for (int i = 4; i >= 0; --i) y = fmaf(u, y, poly[i]);
+    return y * x;
+  }
+
+  template <int N>
+  static __device__ __forceinline__ float largest(const uint32_t* sv) {
+    float big[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < N; c += 2)
+      big[(c >> 1) & 3] = fmaxf(fmaxf(big[(c >> 1) & 3], fabsf(__uint_as_float(sv[c]))), fabsf(__uint_as_float(sv[c + 1])));
+    return fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
+  }
+
   // N products of each thread of a warp become log2(e) softcap tanh(scale s / softcap), or log2(e) scale s without a cap.
   template <int N>
   __device__ __forceinline__ void cap_scores(uint32_t* sv) const {
-    if (capped) {
-      float big[4] = {0.f, 0.f, 0.f, 0.f};
+    if (!capped) {
 #pragma unroll
-      for (int c = 0; c < N; c += 2)
-        big[(c >> 1) & 3] = fmaxf(fmaxf(big[(c >> 1) & 3], fabsf(__uint_as_float(sv[c]))), fabsf(__uint_as_float(sv[c + 1])));
-      const float most = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
+      for (int c = 0; c < N; ++c) sv[c] = __float_as_uint(__uint_as_float(sv[c]) * scale_log2);
+    } else if (!wide) {
+      const float most = largest<N>(sv);
       if (__all_sync(0xffffffffu, most <= near_up_to)) {
         by_polynomial<N, 4>(sv, near);
       } else if (__all_sync(0xffffffffu, most <= poly_up_to)) {
         by_polynomial<N, 6>(sv, poly);
       } else {
 #pragma unroll
-        for (int c = 0; c < N; ++c)
-          sv[c] = __float_as_uint(fmaf(-2.f * cap2, tc::rcp_approx(exp2f(__uint_as_float(sv[c]) * in2) + 1.f), cap2));
+        for (int c = 0; c < N; ++c) sv[c] = __float_as_uint(by_exponential(__uint_as_float(sv[c])));
       }
     } else {
+      // 32 at a time, each with its vote: the branches keep the work on more of them apart, for which there are no registers
 #pragma unroll
-      for (int c = 0; c < N; ++c) sv[c] = __float_as_uint(__uint_as_float(sv[c]) * scale_log2);
+      for (int a = 0; a < N; a += 32) {
+        if (__all_sync(0xffffffffu, largest<32>(sv + a) <= near_up_to)) {
+          by_polynomial<32, 4>(sv + a, near);
+        } else {
+#pragma unroll
+          for (int c = a; c < a + 32; ++c) {
+            const float s = __uint_as_float(sv[c]), y = by_scaled_polynomial(s), z = by_exponential(s);
+            sv[c] = __float_as_uint(fabsf(s) <= wide_up_to ? y : z);
+          }
+        }
+      }
     }
   }
 };
@@ -200,14 +236,23 @@ inline int set_mask(MaskParams* m, const void* rows, const void* tiles, const in
     constexpr double NEAR[4] = {0.9999999019017232, -0.33331362461616354, 0.132709767765151, -0.04755360368917723};
     const double k = static_cast<double>(scale) / softcap, cap2 = softcap * LOG2E;
     double power = cap2 * k;
-    bool fits = true;
+    bool finite = true;
+    int normal = 0;  // coefficients, from the first on
     for (int i = 0; i < 6; ++i, power *= k * k) {
       if (i < 4) m->near[i] = static_cast<float>(NEAR[i] * power);
       m->poly[i] = static_cast<float>(P[i] * power);
-      fits = fits && isfinite(m->poly[i]);
+      finite = finite && isfinite(m->poly[i]);
+      if (normal == i && fabsf(m->poly[i]) >= FLT_MIN) ++normal;
     }
-    m->near_up_to = fits ? static_cast<float>(0.4 / k) : -1.f;
-    m->poly_up_to = fits ? static_cast<float>(0.8 / k) : -1.f;
+    // Without its later coefficients the short form holds as far as they would add less than 2e-8; nor may a square overflow.
+    const double near = normal >= 4 ? 0.4 : normal == 3 ? 0.08 : normal == 2 ? 0.015 : 1e-4;
+    m->near_up_to = finite ? static_cast<float>(fmin(near / k, 1e18)) : -1.f;
+    m->wide = normal < 6;
+    m->poly_up_to = finite && !m->wide ? static_cast<float>(0.8 / k) : -1.f;
+    if (m->wide)
+      for (int i = 0; i < 6; ++i) m->poly[i] = static_cast<float>(P[i] * cap2);
+    m->wide_up_to = static_cast<float>(0.8 / k);
+    m->unit = static_cast<float>(k);
     m->cap2 = static_cast<float>(cap2);
     m->in2 = static_cast<float>(2.0 * LOG2E * k);
     m->neg_inv_cap2_sq = static_cast<float>(-1.0 / (cap2 * cap2));
