@@ -67,3 +67,46 @@ def test_padding_may_hold_anything(bad, cap, slopes):
         assert torch.equal(x, y)
     assert not dirty[0][dead].any() and not dirty[2][dead].any()
     assert (dirty[1].transpose(1, 2)[ids < 0] == -math.inf).all()
+
+
+# ------------------------------------------------------------------ results of a layer norm
+
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_layernorm_in_the_place_of_its_input_has_no_h(device):
+    x, w, res = torch.randn(5, 16, device=device), torch.randn(16, device=device), torch.randn(5, 16, device=device)
+    want, mean, rstd, h = K.layernorm_fwd(x, w)
+    assert h is x or torch.equal(h, x)
+    y = x.clone()
+    out, _, _, h = K.layernorm_fwd(y, w, out=y)
+    assert h is None and out.data_ptr() == y.data_ptr() and torch.equal(y, want)
+    y = x.clone()
+    assert K.layernorm_fwd(y, w, out=y.view(-1).view(5, 16))[3] is None  # the same memory as another tensor
+    y = x.clone()
+    out, _, _, h = K.layernorm_fwd(y, w, res=res, out=y)
+    assert h is not None and torch.equal(h, x + res)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_results_of_a_layernorm_that_share_memory_are_refused(device):
+    T, D = 6, 16
+    buf = torch.randn(4 * T * D, device=device)
+    x, shifted, res = buf[: T * D].view(T, D), buf[D : D + T * D].view(T, D), buf[2 * T * D : 3 * T * D].view(T, D)
+    w, s = torch.randn(D, device=device), torch.randn(T, device=device)
+    fwd = lambda **how: K.layernorm_fwd(x, w, **how)  # noqa: E731
+    free = torch.empty_like(x)
+    for how in ({"out": shifted}, {"res": res, "h_out": shifted}, {"res": res, "out": free, "h_out": free.view(-1).view(T, D)},
+                {"mean": s, "rstd": s.view(1, -1).view(-1)}, {"mean": buf[:T]}, {"rstd": buf[3:3 + T]}):
+        with pytest.raises(ValueError):
+            fwd(**how)
+    with pytest.raises(ValueError):
+        K.layernorm_fwd(x, buf[:D], out=x)  # the weight lies in what is written
+    _, mean, rstd, _ = fwd()
+    dy = torch.randn_like(x)
+    g = torch.empty(D, device=device)
+    for how in ({"dx": shifted}, {"dw": g, "db": g}, {"dw": g, "db": g.view(1, -1).view(-1)}, {"dx": free, "dw": free.view(-1)[:D]}):
+        with pytest.raises(ValueError):
+            K.layernorm_bwd(dy, x, w, mean, rstd, **how)

@@ -126,6 +126,26 @@ void like(const Tensor* t, const char* name, at::ScalarType type, at::IntArrayRe
                     " of shape ", shape, " on ", device, ", got ", t->scalar_type(), " of ", t->sizes(), " on ", t->device());
 }
 
+// Of contiguous tensors: whether they share memory.
+bool overlap(const Tensor* a, const Tensor* b) {
+  if (a == nullptr || b == nullptr || a->numel() == 0 || b->numel() == 0) return false;
+  const auto from = [](const Tensor* t) { return reinterpret_cast<uintptr_t>(t->data_ptr()); };
+  return from(a) < from(b) + b->nbytes() && from(b) < from(a) + a->nbytes();
+}
+
+struct Named {
+  const Tensor* t;
+  const char* name;
+};
+
+// A result is no part of what is read at other times than it is written, and of no other result.  `place`: what it may be written over, as a whole.
+void result_apart(Named r, std::initializer_list<Named> place, std::initializer_list<Named> others) {
+  if (r.t == nullptr) return;
+  for (const Named& o : place)
+    TORCH_CHECK_VALUE(!overlap(r.t, o.t) || r.t->data_ptr() == o.t->data_ptr(), r.name, " may be ", o.name, " as a whole, but no part of its memory");
+  for (const Named& o : others) TORCH_CHECK_VALUE(!overlap(r.t, o.t), r.name, " and ", o.name, " share memory");
+}
+
 void* at_of(const Tensor* t) { return t == nullptr ? nullptr : t->data_ptr(); }
 
 // ------------------------------------------------------------------ spans
@@ -341,7 +361,7 @@ Tensor result(const Tensor* given, at::IntArrayRef shape, at::ScalarType type, a
   return given != nullptr ? *given : empty(shape, type, device);
 }
 
-// (x, w, b or None, eps, then res, h_out, out, mean, rstd or None each) -> (out, mean, rstd, h)
+// (x, w, b or None, eps, then res, h_out, out, mean, rstd or None each) -> (out, mean, rstd, h or None)
 PyObject* layernorm_fwd(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Args a{argv, n};
@@ -361,12 +381,15 @@ PyObject* layernorm_fwd(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   like(b, "b", type, {D}, device);
   like(mean_given, "mean", at::kFloat, {T}, device);
   like(rstd_given, "rstd", at::kFloat, {T}, device);
-  TORCH_CHECK_VALUE(res == nullptr || h_given == nullptr || out_given == nullptr || h_given->data_ptr() != out_given->data_ptr() || T == 0,
-                    "out and h_out are two results");
+  if (res == nullptr) h_given = nullptr;
+  result_apart({out_given, "out"}, {{&x, "x"}, {res, "res"}}, {{h_given, "h_out"}, {&w, "w"}, {b, "b"}, {mean_given, "mean"}, {rstd_given, "rstd"}});
+  result_apart({h_given, "h_out"}, {{&x, "x"}, {res, "res"}}, {{&w, "w"}, {b, "b"}, {mean_given, "mean"}, {rstd_given, "rstd"}});
+  result_apart({mean_given, "mean"}, {}, {{&x, "x"}, {res, "res"}, {&w, "w"}, {b, "b"}, {rstd_given, "rstd"}});
+  result_apart({rstd_given, "rstd"}, {}, {{&x, "x"}, {res, "res"}, {&w, "w"}, {b, "b"}});
   const Stream stream = here(x);
   Tensor out = result(out_given, {T, D}, type, device);
   Tensor mean = result(mean_given, {T}, at::kFloat, device), rstd = result(rstd_given, {T}, at::kFloat, device);
-  Tensor h = res == nullptr ? x : result(h_given, {T, D}, type, device);
+  Tensor h = res != nullptr ? result(h_given, {T, D}, type, device) : overlap(&out, &x) ? Tensor() : x;  // not where out took its place
   if (T > 0)
     launch("layernorm_fwd", entries.layernorm_fwd, x.data_ptr(), at_of(res), res == nullptr ? nullptr : h.data_ptr(), w.data_ptr(), at_of(b),
            out.data_ptr(), mean.data_ptr<float>(), rstd.data_ptr<float>(), T, static_cast<int>(D), static_cast<float>(eps), type == at::kFloat,
@@ -398,6 +421,9 @@ PyObject* layernorm_bwd(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   if (bias) like(db_given, "db", type, {D}, device);
   like(&mean, "mean", at::kFloat, {T}, device);
   like(&rstd, "rstd", at::kFloat, {T}, device);
+  if (!bias) db_given = nullptr;
+  result_apart({dx_given, "dx"}, {{&dy, "dy"}, {&x, "x"}, {dres, "dres"}}, {{&w, "w"}, {&mean, "mean"}, {&rstd, "rstd"}, {dw_given, "dw"}, {db_given, "db"}});
+  result_apart({dw_given, "dw"}, {}, {{db_given, "db"}});
   const Stream stream = here(x);
   Tensor dx = result(dx_given, {T, D}, type, device), dw = result(dw_given, {D}, type, device), db;
   if (bias) db = result(db_given, {D}, type, device);
@@ -417,6 +443,8 @@ PyObject* layernorm_bwd(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   TORCH_CHECK_VALUE(scratch->device() == device && scratch->scalar_type() == at::kFloat && scratch->is_contiguous() && scratch->numel() >= need &&
                         reinterpret_cast<uintptr_t>(scratch->data_ptr()) % 16 == 0,
                     "scratch must be ", need, " contiguous fp32 on ", device);
+  result_apart({scratch, "scratch"}, {}, {{&dy, "dy"}, {&x, "x"}, {dres, "dres"}, {&w, "w"}, {&mean, "mean"}, {&rstd, "rstd"}, {&dx, "dx"}, {&dw, "dw"},
+                                          {bias ? &db : nullptr, "db"}});
   launch("layernorm_bwd", entries.layernorm_bwd, dy.data_ptr(), x.data_ptr(), w.data_ptr(), mean.data_ptr<float>(), rstd.data_ptr<float>(),
          at_of(dres), dx.data_ptr(), dw.data_ptr(), bias ? db.data_ptr() : nullptr, scratch->data_ptr<float>(), T,
          static_cast<int>(D), accumulate, type == at::kFloat, status, stream);

@@ -401,6 +401,21 @@ def _check_norm(x: torch.Tensor) -> None:
         raise ValueError("x must be [rows, width] in bf16 or fp32 with a width that is a multiple of 8")
 
 
+def _result_apart(name: str, r: Optional[torch.Tensor], place: dict, others: dict) -> None:
+    """A result (contiguous, like the others) is no part of what is read at other times than it is written, and of no other result.  ``place``: what
+    it may be written over, as a whole."""
+    if r is None or r.numel() == 0:
+        return
+    for as_a_whole, tensors in ((True, place), (False, others)):
+        for what, t in tensors.items():
+            if t is None or t.numel() == 0 or t.data_ptr() >= r.data_ptr() + r.nbytes or r.data_ptr() >= t.data_ptr() + t.nbytes:
+                continue
+            if not as_a_whole:
+                raise ValueError(f"{name} and {what} share memory")
+            if t.data_ptr() != r.data_ptr():
+                raise ValueError(f"{name} may be {what} as a whole, but no part of its memory")
+
+
 def ref_layernorm_fwd(x, w, b=None, eps=1e-5, res=None):
     h = x.float()
     if res is not None:
@@ -422,10 +437,11 @@ def layernorm_fwd(
     out: Optional[torch.Tensor] = None,
     mean: Optional[torch.Tensor] = None,
     rstd: Optional[torch.Tensor] = None,
-) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
     """Returns ``(normed, mean, rstd, h)`` where ``h = x + res`` (or ``x``), rounded to the type of ``x``, and ``normed = (h - mean) *
     rstd * w (+ b)``.  Rows of up to 16384 elements, all tensors in bf16 or all in fp32 (``mean`` and ``rstd`` in fp32).  ``out`` and
-    ``h_out`` may be ``x`` or ``res``."""
+    ``h_out`` may be ``x`` or ``res`` as a whole; results share no other memory.  Without ``res`` and with ``out`` in the place of ``x``
+    there is no ``h`` any more, and None stands for it."""
     if x.is_cuda:
         results = N.host().layernorm_fwd(x, w, b, eps, res, h_out, out, mean, rstd)
         N.launch_count += x.shape[0] > 0
@@ -444,15 +460,19 @@ def layernorm_fwd(
     _check_like("x res h_out out", dtype, x.shape, at, x, res, h_out, out)
     _check_like("w b", dtype, (D,), at, w, b)
     _check_like("mean rstd", torch.float32, (T,), at, mean, rstd)
-    if out is h_out and res is not None:
-        raise ValueError("out and h_out are two results")
+    inputs, rows = {"x": x, "res": res}, {"w": w, "b": b, "mean": mean, "rstd": rstd}
+    _result_apart("out", out, inputs, {**rows, "h_out": h_out if res is not None else None})
+    _result_apart("h_out", h_out if res is not None else None, inputs, rows)
+    _result_apart("mean", mean, {}, {**inputs, "w": w, "b": b, "rstd": rstd})
+    _result_apart("rstd", rstd, {}, {**inputs, "w": w, "b": b})
+    gone = res is None and out.data_ptr() == x.data_ptr() and x.numel() > 0
     o, m, r, h = ref_layernorm_fwd(x, w, b, eps, res)
     out.copy_(o)
     mean.copy_(m)
     rstd.copy_(r)
     if res is not None:
         h_out.copy_(h)
-    return out, mean, rstd, h_out if res is not None else x
+    return out, mean, rstd, h_out if res is not None else None if gone else x
 
 
 def ref_layernorm_bwd(dy, x, w, mean, rstd, dres=None):
@@ -488,7 +508,7 @@ def layernorm_bwd(
     scratch: Optional[torch.Tensor] = None,
 ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
     """``(dx, dw, db)`` of :func:`layernorm_fwd`, whose ``h`` is ``x`` here; ``db`` is None without ``bias``.  ``dres`` is added to ``dx``,
-    which may be ``dy``, ``x`` or ``dres``; with ``accumulate`` the sums are added to what ``dw`` and ``db`` hold.  The partial sums lie in
+    which may be ``dy``, ``x`` or ``dres`` as a whole (results share no other memory); with ``accumulate`` the sums are added to what ``dw`` and ``db`` hold.  The partial sums lie in
     ``scratch`` (fp32 on the device, :func:`layernorm_bwd_scratch_floats` of them or more) between the two kernels, by default in memory
     of this call's own."""
     if x.is_cuda:
@@ -511,6 +531,8 @@ def layernorm_bwd(
     _check_like("x dy dres dx", dtype, x.shape, at, x, dy, dres, dx)
     _check_like("w dw db", dtype, (D,), at, w, dw, db)
     _check_like("mean rstd", torch.float32, (T,), at, mean, rstd)
+    _result_apart("dx", dx, {"dy": dy, "x": x, "dres": dres}, {"w": w, "mean": mean, "rstd": rstd, "dw": dw, "db": db})
+    _result_apart("dw", dw, {}, {"db": db})
     if T == 0:
         if not accumulate:
             dw.zero_()
