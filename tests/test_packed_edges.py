@@ -110,3 +110,25 @@ def test_results_of_a_layernorm_that_share_memory_are_refused(device):
     for how in ({"dx": shifted}, {"dw": g, "db": g}, {"dw": g, "db": g.view(1, -1).view(-1)}, {"dx": free, "dw": free.view(-1)[:D]}):
         with pytest.raises(ValueError):
             K.layernorm_bwd(dy, x, w, mean, rstd, **how)
+
+
+# ------------------------------------------------------------------ the same answer on both devices
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_sizes_that_no_kernel_takes_are_refused_everywhere(device):
+    pos = torch.zeros(1, 4, dtype=torch.int32, device=device)
+    for dtype, dim, half in ((torch.bfloat16, 12, False), (torch.bfloat16, 8, True), (torch.bfloat16, 24, True), (torch.float32, 6, False),
+                             (torch.float32, 4, True), (torch.float32, 12, True), (torch.float32, 1028, False), (torch.bfloat16, 0, False)):
+        inv, axis = torch.ones(dim // 2, dtype=torch.float64, device=device), torch.zeros(dim // 2, dtype=torch.int32, device=device)
+        with pytest.raises(ValueError, match="head_dim"):
+            K.rope_axes_(torch.zeros(4, max(dim, 1), dtype=dtype, device=device), pos, inv, axis, 1, dim, half=half)
+    inv, axis = K.rope_axes_freqs([8], 10.0, device)
+    for dtype, width in ((torch.bfloat16, 20), (torch.float32, 18)):
+        with pytest.raises(ValueError, match="apart"):
+            K.rope_axes_(torch.zeros(4, width, dtype=dtype, device=device), pos, inv, axis, 1, 16)
+    x, w = torch.zeros(2, 16392, device=device), torch.zeros(16392, device=device)
+    with pytest.raises(ValueError, match="16384"):
+        K.layernorm_fwd(x, w)
+    with pytest.raises(ValueError, match="16384"):
+        K.layernorm_bwd(x, x, w, x[:, 0].contiguous(), x[:, 0].contiguous())

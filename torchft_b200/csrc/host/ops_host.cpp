@@ -316,10 +316,13 @@ PyObject* rope_axes(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   TORCH_CHECK_VALUE(buf.dim() == 2 && (type == at::kBFloat16 || type == at::kFloat) && (buf.size(1) <= 1 || buf.stride(1) == 1),
                     "buf must be a 2-D bf16 or fp32 tensor with unit inner stride");
   const long long T = buf.size(0), width = buf.size(1);
-  const long long ld = T > 1 ? buf.stride(0) : std::max<long long>(buf.stride(0), width);
-  TORCH_CHECK_VALUE(heads >= 1 && dim >= 2 && dim % 2 == 0 && width >= static_cast<long long>(heads) * dim &&
-                        ld >= static_cast<long long>(heads) * dim,
+  const int vector = type == at::kFloat ? 4 : 8;
+  TORCH_CHECK_VALUE(dim > 0 && dim % (half ? 2 * vector : vector) == 0 && dim <= 1024, "head_dim must be a multiple of ", half ? 2 * vector : vector,
+                    " up to 1024 in ", type, half ? ", half-split" : "");
+  const long long ld = T > 1 ? buf.stride(0) : static_cast<long long>(heads) * dim;  // of one row there is none
+  TORCH_CHECK_VALUE(heads >= 1 && heads <= 1 << 20 && width >= static_cast<long long>(heads) * dim && ld >= static_cast<long long>(heads) * dim,
                     "buf of shape ", buf.sizes(), " does not hold ", heads, " heads of ", dim);
+  TORCH_CHECK_VALUE(ld % vector == 0, "the rows of buf must start a multiple of ", vector, " elements apart");
   TORCH_CHECK_VALUE(positions.dim() == 2 && positions.size(0) >= 1 && positions.size(0) <= INT32_MAX, "positions must be contiguous int32 [axes, rows]");
   const at::Device device = buf.device();
   like(&positions, "positions", at::kInt, {positions.size(0), T}, device);
@@ -337,8 +340,8 @@ PyObject* rope_axes(PyObject*, PyObject* const* argv, Py_ssize_t n) {
 
 void norm_rows(const Tensor& x) {
   TORCH_CHECK_VALUE(x.dim() == 2 && (x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kFloat) && x.size(1) % 8 == 0 && x.size(1) > 0 &&
-                        x.size(1) <= INT32_MAX,
-                    "x must be [rows, width] in bf16 or fp32 with a width that is a multiple of 8");
+                        x.size(1) <= 16384,
+                    "x must be [rows, width] in bf16 or fp32 with a width that is a multiple of 8 up to 16384");
 }
 
 PyObject* pack(std::initializer_list<Tensor> ts) {

@@ -397,8 +397,8 @@ def _check_like(names: str, dtype: torch.dtype, shape, device: int, *tensors: Op
 
 
 def _check_norm(x: torch.Tensor) -> None:
-    if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float32) or x.shape[1] % 8 or x.shape[1] == 0:
-        raise ValueError("x must be [rows, width] in bf16 or fp32 with a width that is a multiple of 8")
+    if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float32) or x.shape[1] % 8 or not 0 < x.shape[1] <= 16384:
+        raise ValueError("x must be [rows, width] in bf16 or fp32 with a width that is a multiple of 8 up to 16384")
 
 
 def _result_apart(name: str, r: Optional[torch.Tensor], place: dict, others: dict) -> None:
@@ -624,16 +624,22 @@ def rope_axes_(buf: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tenso
     the rows bring along: pair ``j`` of a head turns by ``positions[axis[j], t] * inv_freq[j]`` (``positions`` int32 ``[axes, T]``,
     ``inv_freq`` fp64 and ``axis`` int32, both ``[head_dim/2]``, see :func:`rope_axes_freqs`); an ``axis`` outside ``[0, axes)`` leaves the
     pair as it is.  Pairs are neighbours, as in :func:`rope_`, or with ``half`` elements ``j`` and ``j + head_dim/2``.  ``backward``
-    turns back."""
+    turns back.  Heads and rows start on 16 bytes: ``head_dim`` is a multiple of 8 in bf16 and of 4 in fp32, with ``half`` of twice that, up
+    to 1024, and so are the rows' strides of 8 and 4."""
     if buf.is_cuda:
         N.launch_count += N.host().rope_axes(buf, positions, inv_freq, axis, n_heads, head_dim, half, backward)
         return buf
     if buf.dim() != 2 or buf.dtype not in (torch.bfloat16, torch.float32) or (buf.shape[1] > 1 and buf.stride(1) != 1):
         raise ValueError("buf must be a 2-D bf16 or fp32 tensor with unit inner stride")
     T = buf.shape[0]
-    ld = buf.stride(0) if T > 1 else max(buf.stride(0), buf.shape[1])
-    if n_heads < 1 or head_dim < 2 or head_dim % 2 or buf.shape[1] < n_heads * head_dim or (T > 1 and ld < n_heads * head_dim):
+    vector = 4 if buf.dtype == torch.float32 else 8
+    if not 0 < head_dim <= 1024 or head_dim % (2 * vector if half else vector):
+        raise ValueError(f"head_dim must be a multiple of {2 * vector if half else vector} up to 1024 in {buf.dtype}{', half-split' if half else ''}")
+    ld = buf.stride(0) if T > 1 else n_heads * head_dim  # of one row there is none
+    if not 1 <= n_heads <= 1 << 20 or buf.shape[1] < n_heads * head_dim or ld < n_heads * head_dim:
         raise ValueError(f"buf of shape {tuple(buf.shape)} does not hold {n_heads} heads of {head_dim}")
+    if ld % vector:
+        raise ValueError(f"the rows of buf must start a multiple of {vector} elements apart")
     if positions.dim() != 2 or positions.shape[0] < 1:
         raise ValueError("positions must be contiguous int32 [axes, rows]")
     at = buf.get_device()
