@@ -132,3 +132,44 @@ def test_sizes_that_no_kernel_takes_are_refused_everywhere(device):
         K.layernorm_fwd(x, w)
     with pytest.raises(ValueError, match="16384"):
         K.layernorm_bwd(x, x, w, x[:, 0].contiguous(), x[:, 0].contiguous())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_rows_that_share_memory_are_refused(device):
+    B, S, H, D = 1, 4, 2, 64
+    q = torch.zeros(S, H * D, dtype=torch.bfloat16, device=device)
+    same = torch.zeros(1, H * D, dtype=torch.bfloat16, device=device).expand(S, H * D)
+    lse = torch.zeros(B, H, S, device=device)
+    for args in ((same, q, q, q), (q, same, q, q), (q, q, same, q), (q, q, q, same)):
+        with pytest.raises(ValueError, match="apart"):
+            K.attention_fwd(*args[:3], B, S, H, H, D, args[3], lse, softcap=10.0)
+    for i in range(8):
+        args = [q] * 8
+        args[i] = same
+        with pytest.raises(ValueError, match="apart"):
+            K.attention_bwd(*args[:5], lse, *args[5:], B, S, H, H, D, softcap=10.0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_one_row_has_no_stride(device):
+    """What a single row's stride says means nothing: a column of another tensor, a width that is no multiple."""
+    H, D = 2, 64
+    g = torch.Generator().manual_seed(0)
+    qkv = [torch.randn(H * D, 1, generator=g).to(device, torch.bfloat16) for _ in range(4)]
+    flat = [t.view(1, -1) for t in qkv]
+    odd = [t.t() for t in qkv]  # strides (1, 1)
+    want, got = torch.empty_like(flat[0]), torch.empty(H * D, 1, dtype=torch.bfloat16, device=device).t()
+    lse = torch.empty(1, H, 1, device=device)
+    K.attention_fwd(*flat[:3], 1, 1, H, H, D, want, lse, softcap=10.0)
+    K.attention_fwd(*odd[:3], 1, 1, H, H, D, got, lse, softcap=10.0)
+    assert torch.equal(got, want)
+    d, e = [torch.empty_like(t) for t in flat[:3]], [torch.empty(H * D, 1, dtype=torch.bfloat16, device=device).t() for _ in range(3)]
+    K.attention_bwd(*flat[:3], want, flat[3], lse, *d, 1, 1, H, H, D, softcap=10.0)
+    K.attention_bwd(*odd[:3], got, odd[3], lse, *e, 1, 1, H, H, D, softcap=10.0)
+    assert all(torch.equal(x, y) for x, y in zip(d, e))
+    inv, axis = K.rope_axes_freqs([8], 10.0, device)
+    pos = torch.tensor([[5]], dtype=torch.int32, device=device)
+    buf = torch.randn(1, 2 * 16 + 3, generator=g).to(device)
+    even = buf[:, :32].contiguous()
+    K.rope_axes_(buf, pos, inv, axis, 2, 16)
+    assert torch.equal(buf[:, :32], K.rope_axes_(even, pos, inv, axis, 2, 16))

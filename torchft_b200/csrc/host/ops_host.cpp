@@ -219,10 +219,13 @@ struct Mask {
   // a [batch * seq, n * dim] view of bf16
   void view(const Tensor& t, const char* name, int n, at::Device device) const {
     TORCH_CHECK_VALUE(t.dim() == 2 && t.size(0) == static_cast<long long>(batch) * seq && t.size(1) == static_cast<long long>(n) * dim &&
-                          t.scalar_type() == at::kBFloat16 && t.stride(1) == 1 && t.device() == device,
-                      name, " must be bf16 [", static_cast<long long>(batch) * seq, ", ", n * dim, "] with unit inner stride on ", device, ", got ",
-                      t.scalar_type(), " of ", t.sizes(), " on ", t.device());
+                          t.scalar_type() == at::kBFloat16 && t.stride(1) == 1 && t.device() == device &&
+                          (t.size(0) <= 1 || t.stride(0) >= t.size(1)),
+                      name, " must be bf16 [", static_cast<long long>(batch) * seq, ", ", n * dim, "] with unit inner stride, its rows apart, on ", device,
+                      ", got ", t.scalar_type(), " of ", t.sizes(), ", strides ", t.strides(), ", on ", t.device());
   }
+  // Between rows; of one there is none.
+  static long long ld(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
   void rest(const Tensor* lse, at::Device device) {
     like(slopes, "slopes", at::kFloat, {heads}, device);
     like(lse, "lse", at::kFloat, {batch, heads, seq}, device);
@@ -256,7 +259,7 @@ PyObject* attention_masked_fwd(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   const Stream stream = here(q);
   if (m.batch == 0 || m.seq == 0) return PyLong_FromLong(0);
   launch("attention_masked_fwd", entries.masked_fwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), static_cast<float*>(at_of(lse)),
-         m.rows, m.tiles, m.padded, m.slopes_at(), m.batch, m.seq, m.heads, m.kv_heads, m.dim, q.stride(0), k.stride(0), v.stride(0), out.stride(0),
+         m.rows, m.tiles, m.padded, m.slopes_at(), m.batch, m.seq, m.heads, m.kv_heads, m.dim, m.ld(q), m.ld(k), m.ld(v), m.ld(out),
          m.scale(), m.cap, m.causal, status, stream);
   return PyLong_FromLong(1);
   END_HANDLE_TH_ERRORS
@@ -297,7 +300,7 @@ PyObject* attention_masked_bwd(PyObject*, PyObject* const* argv, Py_ssize_t n) {
                     "scratch must be ", need, " contiguous bytes on ", device);
   launch("attention_masked_bwd", entries.masked_bwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), d_o.data_ptr(), lse.data_ptr<float>(),
          dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), scratch->data_ptr(), m.rows, m.tiles, m.padded, m.slopes_at(), m.batch, m.seq, m.heads,
-         m.kv_heads, m.dim, q.stride(0), k.stride(0), v.stride(0), o.stride(0), d_o.stride(0), dq.stride(0), dk.stride(0), dv.stride(0), m.scale(),
+         m.kv_heads, m.dim, m.ld(q), m.ld(k), m.ld(v), m.ld(o), m.ld(d_o), m.ld(dq), m.ld(dk), m.ld(dv), m.scale(),
          m.cap, m.causal, static_cast<const float*>(at_of(rope)), status, stream);
   return PyLong_FromLong(3);
   END_HANDLE_TH_ERRORS

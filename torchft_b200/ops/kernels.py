@@ -1030,9 +1030,9 @@ def _check_masked(of_q, of_kv, spans: Optional[AttentionSpans], softcap: float, 
     for tensors, heads in ((of_q, n_heads), (of_kv, n_kv_heads)):
         shape = (batch * seq_len, heads * head_dim)
         for t in tensors:
-            if t.shape != shape or t.dtype != torch.bfloat16 or t.stride(1) != 1 or t.get_device() != at:
-                raise ValueError(f"a tensor of {heads} heads must be bf16 {shape} with unit inner stride on {of_q[0].device}, got {t.dtype} "
-                                 f"{tuple(t.shape)} on {t.device}")
+            if t.shape != shape or t.dtype != torch.bfloat16 or t.stride(1) != 1 or t.get_device() != at or (shape[0] > 1 and t.stride(0) < shape[1]):
+                raise ValueError(f"a tensor of {heads} heads must be bf16 {shape} with unit inner stride, its rows apart, on {of_q[0].device}, got "
+                                 f"{t.dtype} {tuple(t.shape)}, strides {t.stride()}, on {t.device}")
     if softcap != 0.0 and not 1e-9 <= softcap <= 1e30:
         raise ValueError("softcap must be 0 or a cap from 1e-9 to 1e30")
     if spans is not None and (spans.batch, spans.seq) != (batch, seq_len):
