@@ -5,8 +5,9 @@ with the source tree:
 
 * ``torchft_b200/_lib/libftb200_kernels.so`` -- every hand-written sm_100a CUDA
   kernel, exported through a plain C ABI (loaded with ``ctypes``).
-* ``torchft_b200/_ops_host.<ext-suffix>.so`` -- argument checks, result tensors and calls
-  of some operators in one C++ call each (a CPython module against torch's headers).
+* ``torchft_b200/_ops_host_<torch>.<ext-suffix>.so`` -- argument checks, result tensors and calls
+  of some operators in one C++ call each (a CPython module against torch's headers, good for the build of
+  torch that its name stands for).
 * ``torchft_b200/_ftcp.<ext-suffix>.so``   -- the C++ control plane (lighthouse,
   manager server/client, quorum math) as a pybind11 module.
 
@@ -39,7 +40,6 @@ BUILD_DIR = REPO_DIR / "build"
 KERNEL_LIB = LIB_DIR / "libftb200_kernels.so"
 KERNEL_LIB_CHECKED = LIB_DIR / "libftb200_kernels_checked.so"  # -DFT_BOUNDS_CHECK=1 debug build
 CONTROL_MOD = PKG_DIR / ("_ftcp" + sysconfig.get_config_var("EXT_SUFFIX"))
-HOST_MOD = PKG_DIR / ("_ops_host" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 NVCC_FLAGS = [
     "-gencode",
@@ -179,14 +179,25 @@ def build_control() -> Path:
         return CONTROL_MOD
 
 
+def _torch_dir() -> Path:
+    spec = importlib.util.find_spec("torch")  # found, not imported
+    if spec is None or not spec.submodule_search_locations:
+        raise RuntimeError("torch not found; cannot build torchft_b200's host module")
+    return Path(spec.submodule_search_locations[0])
+
+
+def host_mod() -> Path:
+    """Where the host module for the torch that is installed lies.  It uses more of torch than its stable interface, so
+    that one built against another version, commit or CUDA is not loaded."""
+    torch_build = hashlib.sha256((_torch_dir() / "version.py").read_bytes()).hexdigest()[:12]
+    return PKG_DIR / f"_ops_host_{torch_build}{sysconfig.get_config_var('EXT_SUFFIX')}"
+
+
 def build_host() -> Path:
     """Compile the host side of the operators that have one in C++.  torch's libraries are found where ``import torch``
     has loaded them, so the module carries no path of theirs."""
     with _lock:
-        spec = importlib.util.find_spec("torch")  # found, not imported
-        if spec is None or not spec.submodule_search_locations:
-            raise RuntimeError("torch not found; cannot build torchft_b200's host module")
-        torch_dir = Path(spec.submodule_search_locations[0])
+        torch_dir, target = _torch_dir(), host_mod()
         sources = sorted((CSRC / "host").glob("*.cpp"))
         flags = [
             "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall",
@@ -196,10 +207,10 @@ def build_host() -> Path:
             f"-I{_cuda_home()}/include",
         ]
         objs = _compile_objects(sources, [torch_dir / "version.py"], ["g++"], flags, "h")  # another torch: compiled again
-        if _needs_link(HOST_MOD, objs):
+        if _needs_link(target, objs):
             libs = ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python"]
-            _run(["g++", "-shared", "-o", str(HOST_MOD), *map(str, objs), f"-L{torch_dir / 'lib'}", *libs])
-        return HOST_MOD
+            _run(["g++", "-shared", "-o", str(target), *map(str, objs), f"-L{torch_dir / 'lib'}", *libs])
+        return target
 
 
 def build_all(verbose: bool = False) -> None:
@@ -211,4 +222,4 @@ def build_all(verbose: bool = False) -> None:
 
 if __name__ == "__main__":
     build_all(verbose="-v" in sys.argv)
-    print("built:", KERNEL_LIB, CONTROL_MOD)
+    print("built:", KERNEL_LIB, CONTROL_MOD, host_mod())

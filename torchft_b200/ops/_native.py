@@ -8,7 +8,8 @@ that no GPU code path silently falls back to eager PyTorch.
 from __future__ import annotations
 
 import ctypes
-import importlib
+import importlib.machinery
+import importlib.util
 import os
 import threading
 from typing import Optional
@@ -90,19 +91,22 @@ _HOST_ENTRIES = ("attention_spans", "attention_masked_fwd", "attention_masked_bw
 
 
 def host():
-    """The C++ host side of some operators (``torchft_b200/_ops_host``), bound to the library of :func:`lib`.  Like that
-    it is mandatory where those operators run on a GPU."""
+    """The C++ host side of some operators (``torchft_b200/_ops_host_*.so`` of the torch that is installed), bound to the
+    library of :func:`lib`.  Like that it is mandatory where those operators run on a GPU."""
     global _host
     if _host is not None:
         return _host
     library = lib()
     with _lock:
         if _host is None:
-            if not _build.HOST_MOD.exists():
+            path = _build.host_mod()
+            if not path.exists():
                 if os.environ.get("FTB200_NO_AUTOBUILD"):
-                    raise KernelError(f"{_build.HOST_MOD} is missing; run `python -m torchft_b200._build`")
+                    raise KernelError(f"{path} is missing; run `python -m torchft_b200._build`")
                 _build.build_host()
-            module = importlib.import_module("torchft_b200._ops_host")
+            loader = importlib.machinery.ExtensionFileLoader("torchft_b200._ops_host", str(path))
+            module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("torchft_b200._ops_host", path, loader=loader))
+            loader.exec_module(module)
             module.bind(check_host, *(ctypes.cast(getattr(library, "ftb200_" + e), c_void_p).value for e in _HOST_ENTRIES))
             _host = module
         return _host
