@@ -1,5 +1,5 @@
 """Regenerate ``docs/api.md``: the public classes and functions of every user-facing module with their
-signatures and the first paragraph of their docstrings.
+signatures and their docstrings: the first paragraph of a module's, a class's or a method's, all of a function's.
 
     python docs/gen_api.py            # rewrite docs/api.md
     python docs/gen_api.py --check    # exit 1 if docs/api.md is out of date
@@ -59,6 +59,11 @@ def _first_paragraph(obj) -> str:
     doc = inspect.cleandoc(getattr(obj, "__doc__", None) or "") if not isinstance(obj, property) else inspect.cleandoc(obj.__doc__ or "")
     para = doc.split("\n\n", 1)[0].strip()
     return " ".join(line.strip() for line in para.splitlines())
+
+
+def _paragraphs(obj) -> list:
+    doc = inspect.cleandoc(getattr(obj, "__doc__", None) or "")
+    return [" ".join(line.strip() for line in para.splitlines()) for para in doc.split("\n\n") if para.strip()]
 
 
 def _bound_signature(obj) -> str:
@@ -125,8 +130,7 @@ def render() -> str:
             elif callable(obj):
                 out.append(f"### `{name}{_signature(obj)}`")
                 out.append("")
-                d = _first_paragraph(obj)
-                if d:
+                for d in _paragraphs(obj):
                     out += [d, ""]
     return "\n".join(out).rstrip() + "\n"
 

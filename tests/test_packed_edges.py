@@ -173,3 +173,11 @@ def test_one_row_has_no_stride(device):
     even = buf[:, :32].contiguous()
     K.rope_axes_(buf, pos, inv, axis, 2, 16)
     assert torch.equal(buf[:, :32], K.rope_axes_(even, pos, inv, axis, 2, 16))
+
+
+def test_the_reference_page_explains_every_argument_of_a_mask():
+    page = (_build.REPO_DIR / "docs" / "api.md").read_text()
+    for name in ("attention_fwd", "attention_bwd", "attention_spans"):
+        text = page.split(f"### `{name}(", 1)[1].split("\n", 1)[1].split("\n### ", 1)[0]
+        for arg in ("documents", "prefix", "causal", "window") if name == "attention_spans" else ("spans", "softcap", "slopes"):
+            assert f"``{arg}``" in text, (name, arg)

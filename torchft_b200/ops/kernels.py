@@ -1162,7 +1162,8 @@ def attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Te
     ``any_length``, of any length.
 
     ``spans``, ``softcap`` and ``slopes`` as in the forward pass; with any of them sequences have any length, the default
-    ``scratch`` is this call's own, and rows that see nothing, or are seen by nobody, get zeros."""
+    ``scratch`` is this call's own, and rows that see nothing, or are seen by nobody, get zeros.  Probabilities are made again from the
+    fp32 ``lse`` and are off by about 2^-22 of the score's size, so that from scores of 10^5 on the gradients lose their meaning."""
     if spans is not None or softcap != 0.0 or slopes is not None:
         if q.is_cuda:
             if spans is not None and (spans.batch != batch or spans.seq != seq_len):
