@@ -524,7 +524,10 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       const ulonglong2* delta2 = lse2 + BQ / 4;
       float pe[CPT];
       if constexpr (SCORE) {
-        uint32_t sv[32];
+        uint32_t both[2][32];  // the second half on its way under the first; capped all at once two words of a thread would go to local memory
+        tmem_ld32(s_addr, both[0]);
+        tmem_wait_ld();
+        tmem_ld32(s_addr + 32, both[1]);
         const float slope2 = p.mask.slope2(w.h);
         const float far = static_cast<float>(w.qt * BQ + g * CPT - (jb * BKV + row));
         const bool all = __all_sync(0xffffffffu, mine.all(w.qt * BQ, BQ));  // the same in all lanes; said so, as whole warps access tensor memory below
@@ -534,8 +537,8 @@ attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           for (int half = 0; half < 2; ++half) {
             const int q0 = w.qt * BQ + g * CPT + half * 32;
             const uint32_t bits = decltype(partial)::value ? ftb200::range_bits(mine.lo - q0, mine.hi - q0) : 0u;
-            tmem_ld32(s_addr + half * 32, sv);  // (with both halves in registers two words of a thread would go to local memory)
-            tmem_wait_ld();
+            uint32_t* sv = both[half];
+            if (half == 1) tmem_wait_ld();
             p.mask.cap_scores<32>(sv);
             uint32_t pt[16];
 #pragma unroll

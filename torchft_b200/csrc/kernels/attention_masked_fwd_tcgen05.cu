@@ -313,7 +313,7 @@ attention_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
           }
           if (j == 0 && full > 0 && !wait(BAR_O_FREE + t, full - 1)) return false;
           const uint32_t vb = same(v_lo + st * STAGE16);
-#pragma unroll 1
+#pragma unroll (C::OWN_P ? 2 : 1)  // at head dim 128 both at once would put a word in local memory
           for (int half = 0; half < 2; ++half) {
             if (!wait((half == 0 ? BAR_P_HALF : BAR_P_FULL) + t, g)) return false;
             tc_fence_after();

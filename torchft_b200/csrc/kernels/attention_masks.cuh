@@ -131,11 +131,19 @@ struct MaskParams {
   // become zeros, by one warp: what stands in padding may be anything, and zero times infinity would reach the tile's other rows.  The
   // products that follow see it.
   __device__ __forceinline__ void clear_padding(uint32_t tile_addr, int slabs, int b, int first, int seq, int lane) const {
-    for (int r = lane; r < 128 && first + r < seq; r += 32) {
-      const KeyRange x = row(b, first + r, seq);
-      if (x.hi > x.lo) continue;
-      const uint32_t at = tile_addr + r * 128;
-      for (int c = 0; c < slabs * 8; ++c) tc::st_shared_zero16(at + (c >> 3) * (128 * 128) + (c & 7) * 16);
+    const int2* spans = reinterpret_cast<const int2*>(rows + static_cast<long long>(b) * seq + first + lane);
+    const int rest = seq - first - lane;
+    uint32_t dead = 0;  // all rows are looked up before the first store
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      int2 x = make_int2(0, 1);
+      if (32 * i < rest) x = spans[2 * 32 * i];
+      dead |= static_cast<uint32_t>(x.y <= x.x) << i;
+    }
+    for (int i = 0; dead != 0; ++i, dead >>= 1) {
+      const uint32_t at = tile_addr + (lane + 32 * i) * 128;
+      if (dead & 1u)
+        for (int c = 0; c < slabs * 8; ++c) tc::st_shared_zero16(at + (c >> 3) * (128 * 128) + (c & 7) * 16);
     }
     tc::fence_async_smem();
     __syncwarp();
