@@ -117,3 +117,23 @@ def test_caps_and_scores_beyond_sense(cap, size, D):
     # the largest score, to 2^-21 of its terms and 2^-20 of itself
     want = torch.logsumexp(s, -1)
     assert ((lse.double() - want).abs() <= 2.0**-21 * sizes + 2.0**-20 * want.abs()).all()
+
+
+# ------------------------------------------------------------------ rotation
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_rotation_by_angles_of_more_than_24_bits(half):
+    """Of the pair (1, 0) the cosine and the sine are left, each within two steps of itself: one of the functions, half a one of what is added for the
+    angle's further bits, half a one to spare; the product of position and frequency is off by 2^-53 of itself, thrice."""
+    T, dim, n = 20000, 128, 2
+    g = torch.Generator(device="cuda").manual_seed(3)
+    inv, axis = K.rope_axes_freqs([dim // 2], 10000.0, "cuda")
+    pos = torch.randint(0, 1 << 14, (1, T), dtype=torch.int32, device="cuda", generator=g)
+    buf = torch.zeros(T, n, dim, device="cuda")
+    x, y = (buf[..., : dim // 2], buf[..., dim // 2 :]) if half else (buf[..., 0::2], buf[..., 1::2])
+    x.fill_(1.0)
+    K.rope_axes_(buf.view(T, n * dim), pos, inv, axis, n, dim, half=half)
+    angle = (pos.double().t() * inv)[:, None]
+    for got, want in ((x, angle.cos()), (y, angle.sin())):
+        assert ((got.double() - want).abs() <= 2 * 2.0**-23 * want.abs() + 3 * 2.0**-53 * 2**14).all()

@@ -179,7 +179,8 @@ __global__ void __launch_bounds__(SPAN_THREADS) spans_kernel(const int* document
 // ------------------------------------------------------------------ rotary positions with several axes
 // Pair j of every rotated head of token t turns by positions[axis[j]][t] * inv_freq[j], in place; an axis outside [0, axes) leaves
 // it.  Pairs are neighbours (2j, 2j + 1) or, with HALF, (j, j + dim / 2).  The angle is a product in 64 bits, brought into one turn there:
-// at position 2^20 32 bits are off by 0.06 rad.
+// at position 2^20 32 bits are off by 0.06 rad.  Sine and cosine are those of its first 24 bits, turned on by the rest (to first order: off by
+// 5e-15), so that near a zero they keep their digits; 20000 x 1 head of 256 take 16.1 us for it instead of 15.2, the other shapes the same.
 //
 // Bound by memory.  A block takes `per_block` tokens: each (token, pair) has its sine taken once, into shared memory, while the first
 // vectors are on their way, and serves all heads.  A thread keeps its place in the head and steps over heads and tokens, without a division.
@@ -248,7 +249,11 @@ __global__ void __launch_bounds__(ROPE_THREADS, 4) rope_axes_kernel(T* buf, cons
     float2 cs = make_float2(1.f, 0.f);
     if (a >= 0 && a < axes) {
       const double turns = static_cast<double>(positions[a * tokens + t0 + token]) * inv_freq[j] * 0.15915494309189534;  // 1 / 2 pi
-      sincospif(2.f * static_cast<float>(turns - rint(turns)), &cs.y, &cs.x);
+      const double halves = 2.0 * (turns - rint(turns));
+      const float near = static_cast<float>(halves), rest = static_cast<float>(halves - near) * 3.14159265f;  // of 24 bits, and what they leave
+      float sine, cosine;
+      sincospif(near, &sine, &cosine);
+      cs = make_float2(fmaf(-rest, sine, cosine), fmaf(rest, cosine, sine));
     }
     turn[i] = cs;
   }
