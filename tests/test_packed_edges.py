@@ -181,3 +181,15 @@ def test_the_reference_page_explains_every_argument_of_a_mask():
         text = page.split(f"### `{name}(", 1)[1].split("\n", 1)[1].split("\n### ", 1)[0]
         for arg in ("documents", "prefix", "causal", "window") if name == "attention_spans" else ("spans", "softcap", "slopes"):
             assert f"``{arg}``" in text, (name, arg)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_table_of_other_positions_is_refused(device):
+    B, S, H, D = 1, 6, 2, 64
+    q, lse = torch.zeros(B * S, H * D, dtype=torch.bfloat16, device=device), torch.zeros(B, H, S, device=device)
+    call = lambda rope: K.attention_bwd(q, q, q, q, q, lse, *(torch.empty_like(q) for _ in range(3)), B, S, H, H, D, softcap=9.0, rope=rope)  # noqa: E731
+    table = K.rope_table(S, D, 1e4, device)
+    call(table)
+    for bad in (table[:-1], table[:, :-1], table.double(), table.transpose(0, 1), table[0]):
+        with pytest.raises(ValueError, match="rope"):
+            call(bad)

@@ -1173,6 +1173,9 @@ def attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Te
                 head_dim, softcap, causal, _status_ptr(q.device))
             return
         _check_masked((q, o, d_o, dq), (k, v, dk, dv), spans, softcap, slopes, lse, batch, seq_len, n_heads, n_kv_heads, head_dim)
+        if rope is not None and (rope.dtype != torch.float32 or not rope.is_contiguous() or rope.get_device() != q.get_device() or rope.dim() != 3
+                                 or rope.shape[0] < seq_len or rope.shape[1:] != (head_dim // 2, 2)):
+            raise ValueError("rope must be the table of the sequence and head dim on the device of q")
         if batch == 0 or seq_len == 0:
             return
         q4, k4, v4 = (t.detach().reshape(batch, seq_len, -1, head_dim).float().requires_grad_(True) for t in (q, k, v))
