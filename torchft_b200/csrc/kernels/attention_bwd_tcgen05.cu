@@ -43,8 +43,12 @@
 // With MASK a key is seen by a range of queries of its own (attention_masks.cuh), so a block walks over the query tiles of that range only, and
 // a softmax thread, whose key it is, holds the range's ends.  With SCORE the scores were capped or lowered by their distance, which is done
 // again here, and dS gets the factor 1 - tanh^2 by way of P, once dV's operand has been made of it.
-// 1 x 8192, 32/8 heads of 128, all three launches: causal with a cap 1315 us (1045 TFLOP/s), with slopes 1190; documents of 1000 tokens on average 311 (595
+// 1 x 8192, 32/8 heads of 128, all three launches: causal with a cap 1333 us (1030 TFLOP/s), with slopes 1182; documents of 1000 tokens on average 309 (599
 // TFLOP/s of the pairs that are seen; their blocks hold 1.3 times as many), of which 43 clear dQ's sums and read O and dO, at the rate of a copy.
+//
+// Roundings to bf16: P^T and dS^T, as the tensor cores take them next to dO, Q and K (up to 2^-8 of each element), and delta is the product of dO with the O
+// that was stored, not with the fp32 one, which nobody keeps.  Gradients are off by 2.6e-3 of their norm, where
+// fp32 operands and one rounding at the end leave 1.7e-3.  Sums, statistics and dQ's accumulator are fp32.
 //
 // Every mbarrier wait is bounded; on expiry the CTA records FTB200_ST_TIMEOUT in the caller's
 // status word, frees its TMEM and returns.

@@ -31,8 +31,8 @@
 // Sequences of any length: the tensor maps have the sequence as a dimension of its own, so a tile's rows beyond its end are zeros (not the
 // next sequence's); keys there are in no query's range, queries there are not stored.
 //
-// 1 x 8192, 32/8 heads of 128: documents of 1000 tokens on average 113 us (658 TFLOP/s of the pairs that are seen), with a cap 147; causal with a
-// cap 603 (912 TFLOP/s; 434 in the kernel without masks and caps), with slopes 525 (659 with the first block first).
+// 1 x 8192, 32/8 heads of 128: documents of 1000 tokens on average 113 us (655 TFLOP/s of the pairs that are seen), with a cap 145; causal with a
+// cap 611 (900 TFLOP/s; 441 in the kernel without masks and caps), with slopes 503 (659 with the first block first).
 //
 // Every mbarrier wait is bounded; on expiry the CTA records FTB200_ST_TIMEOUT in the caller's status word, frees its TMEM and returns.
 #include <cuda.h>
@@ -522,6 +522,7 @@ attention_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
             p0 = exp2f(p0);
             p1 = exp2f(p1);
             sum2[e & 1] = f2_add(sum2[e & 1], f2_pack(p0, p1));
+            // to bf16, as the product takes it next to V: off by up to 2^-8 of itself, where the sum, kept in fp32, has it whole
             __nv_bfloat162 pk = __floats2bfloat162_rn(p0, p1);
             packed[e] = *reinterpret_cast<uint32_t*>(&pk);
           }

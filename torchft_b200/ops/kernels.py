@@ -1076,8 +1076,9 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: int,
 
     ``spans`` (:func:`attention_spans`) say which keys a query sees, in place of ``causal``. ``softcap`` caps the scaled scores: ``softcap *
     tanh(s / softcap)`` (a cap from 1e-9 to 1e30); ``slopes`` (fp32 ``[n_heads]``, not differentiated) lower them by ``slope * |query -
-    key|``. With any of the three the sequence may have any length; a row that sees nothing gets zeros and a ``lse`` of -infinity. Keys of
-    another document that share a block of 128 with those of a row have to be finite; padding need not."""
+    key|``. With any of the three the sequence may have any length; a row that sees nothing gets zeros and a ``lse`` of -infinity. Keys and
+    values that a row does not see, of another document or behind it, have to be finite where they share a block of 128 with some that it
+    sees; padding need not."""
     if spans is not None or softcap != 0.0 or slopes is not None:
         if q.is_cuda:
             if spans is not None and (spans.batch != batch or spans.seq != seq_len):
