@@ -98,6 +98,29 @@ def test_caps_of_every_size(cap, most, D):
 
 
 @pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("form,power", [((0.0475536, 0.0531143), 3), ((0.1327098, 0.1332105), 2)])
+def test_caps_where_one_form_loses_a_coefficient_and_the_other_does_not(form, power, D):
+    """Coefficient c_i of a form is c_i log2(e) cap (scale / cap)^(2 i + 1): at this cap the shorter form's is below the normal fp32 numbers."""
+    scale = D**-0.5
+    low, high = ((c * 1.442695 * scale ** (2 * power + 1) / torch.finfo(torch.float32).tiny) ** (1 / (2 * power)) for c in form)
+    cap = (low * high) ** 0.5
+    assert low < cap < high
+    B, S, H, G = 1, 200, 2, 1
+    q, k, v, _ = _spread(B, S, H, G, D, 10.0, 7)
+    q = (q.double() * (cap / 60)).bfloat16()  # the largest scores about a third of the cap
+    flat = lambda t: t.reshape(B * S, -1)  # noqa: E731
+    out, lse = torch.empty_like(flat(q)), torch.empty(B, H, S, device="cuda")
+    K.attention_fwd(flat(q), flat(k), flat(v), B, S, H, G, D, out, lse, softcap=cap)
+    K.check_status(q.device)
+    q, k = q.double().transpose(1, 2), k.double().transpose(1, 2).repeat_interleave(H // G, 1)
+    s = (cap * torch.tanh(q @ k.transpose(-1, -2) * scale / cap)).masked_fill(~torch.ones(S, S, dtype=torch.bool, device="cuda").tril(), -math.inf)
+    assert 0.1 * cap < s.max() < 0.4 * cap  # the short form's
+    sizes = (q.abs() @ k.abs().transpose(-1, -2)).amax(-1) * scale
+    want = torch.logsumexp(s, -1)
+    assert ((lse.double() - want).abs() <= 2.0**-21 * sizes + 2.0**-20 * want.abs()).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("size", [0.05, 1.0])
 @pytest.mark.parametrize("cap", [1e12, 1e20, 1e30])
 def test_caps_and_scores_beyond_sense(cap, size, D):

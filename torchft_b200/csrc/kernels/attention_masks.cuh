@@ -250,7 +250,7 @@ inline int set_mask(MaskParams* m, const void* rows, const void* tiles, const in
       if (i < 4) m->near[i] = static_cast<float>(NEAR[i] * power);
       m->poly[i] = static_cast<float>(P[i] * power);
       finite = finite && isfinite(m->poly[i]);
-      if (normal == i && fabsf(m->poly[i]) >= FLT_MIN) ++normal;
+      if (normal == i && fabsf(m->poly[i]) >= FLT_MIN && (i >= 4 || fabsf(m->near[i]) >= FLT_MIN)) ++normal;
     }
     // Without its later coefficients the short form holds as far as they would add less than 2e-8; nor may a square overflow.
     const double near = normal >= 4 ? 0.4 : normal == 3 ? 0.08 : normal == 2 ? 0.015 : 1e-4;
