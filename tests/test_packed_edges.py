@@ -107,7 +107,7 @@ def test_results_of_a_layernorm_that_share_memory_are_refused(device):
     _, mean, rstd, _ = fwd()
     dy = torch.randn_like(x)
     g = torch.empty(D, device=device)
-    for how in ({"dx": shifted}, {"dw": g, "db": g}, {"dw": g, "db": g.view(1, -1).view(-1)}, {"dx": free, "dw": free.view(-1)[:D]}):
+    for how in ({"dx": shifted}, {"dw": w}, {"db": dy[0]}, {"dw": g, "db": g}, {"dw": g, "db": g.view(1, -1).view(-1)}, {"dx": free, "dw": free.view(-1)[:D]}):
         with pytest.raises(ValueError):
             K.layernorm_bwd(dy, x, w, mean, rstd, **how)
 

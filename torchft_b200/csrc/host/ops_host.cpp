@@ -429,6 +429,8 @@ PyObject* layernorm_bwd(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   like(&rstd, "rstd", at::kFloat, {T}, device);
   if (!bias) db_given = nullptr;
   result_apart({dx_given, "dx"}, {{&dy, "dy"}, {&x, "x"}, {dres, "dres"}}, {{&w, "w"}, {&mean, "mean"}, {&rstd, "rstd"}, {dw_given, "dw"}, {db_given, "db"}});
+  for (const Named& sums : {Named{dw_given, "dw"}, Named{db_given, "db"}})
+    result_apart(sums, {}, {{&dy, "dy"}, {&x, "x"}, {dres, "dres"}, {&w, "w"}, {&mean, "mean"}, {&rstd, "rstd"}});
   result_apart({dw_given, "dw"}, {}, {{db_given, "db"}});
   const Stream stream = here(x);
   Tensor dx = result(dx_given, {T, D}, type, device), dw = result(dw_given, {D}, type, device), db;

@@ -532,6 +532,8 @@ def layernorm_bwd(
     _check_like("w dw db", dtype, (D,), at, w, dw, db)
     _check_like("mean rstd", torch.float32, (T,), at, mean, rstd)
     _result_apart("dx", dx, {"dy": dy, "x": x, "dres": dres}, {"w": w, "mean": mean, "rstd": rstd, "dw": dw, "db": db})
+    for name, t in (("dw", dw), ("db", db)):
+        _result_apart(name, t, {}, {"dy": dy, "x": x, "dres": dres, "w": w, "mean": mean, "rstd": rstd})
     _result_apart("dw", dw, {}, {"db": db})
     if T == 0:
         if not accumulate:
