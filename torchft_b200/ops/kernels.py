@@ -508,9 +508,9 @@ def layernorm_bwd(
     scratch: Optional[torch.Tensor] = None,
 ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
     """``(dx, dw, db)`` of :func:`layernorm_fwd`, whose ``h`` is ``x`` here; ``db`` is None without ``bias``.  ``dres`` is added to ``dx``,
-    which may be ``dy``, ``x`` or ``dres`` as a whole (results share no other memory); with ``accumulate`` the sums are added to what ``dw`` and ``db`` hold.  The partial sums lie in
-    ``scratch`` (fp32 on the device, :func:`layernorm_bwd_scratch_floats` of them or more) between the two kernels, by default in memory
-    of this call's own."""
+    which may be ``dy``, ``x`` or ``dres`` as a whole (results share no other memory); with ``accumulate`` the sums are added to what ``dw``
+    and ``db`` hold.  The partial sums lie in ``scratch`` (fp32 on the device, :func:`layernorm_bwd_scratch_floats` of them or more) between
+    the two kernels, by default in memory of this call's own."""
     if x.is_cuda:
         results = N.host().layernorm_bwd(dy, x, w, mean, rstd, dres, dx, dw, db, bias, accumulate, scratch, _status_ptr(x.device))
         N.launch_count += 2 * (x.shape[0] > 0)
